@@ -120,7 +120,9 @@ def hipcc_path() -> Optional[str]:
     return None
 
 
-HIPCC_FLAGS = ("--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result")
+# packed fp32 instructions (v_pk_fma_f32 and its like) stay off: some of their forms have given wrong results on these machines
+HIPCC_FLAGS = ("--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result",
+               "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops")
 OBJ_DIR = os.path.join(CSRC, "build")      # per-source objects + the key each was compiled under (git-ignored)
 
 

@@ -29,7 +29,7 @@ __device__ __forceinline__ csn_v2 csn_fmav2(csn_v2 a, csn_v2 b, csn_v2 c) { retu
 #else
 typedef float csn_v2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ csn_v2 csn_mk2(float a, float b) { csn_v2 r = {a, b}; return r; }
-__device__ __forceinline__ csn_v2 csn_fma2(float w, csn_v2 x, csn_v2 c) {   // v_pk_fma_f32
+__device__ __forceinline__ csn_v2 csn_fma2(float w, csn_v2 x, csn_v2 c) {   // two v_fma_f32: packed fp32 instructions are off in every build
   const csn_v2 ww = {w, w};
   return __builtin_elementwise_fma(ww, x, c);
 }

@@ -98,7 +98,7 @@ __global__ __launch_bounds__(CSN_BLOCK) void msblock_kernel(MsArgs a) {
 // msr_kernel: four pixels per lane with vertical reuse.  A lane owns QUADS of four consecutive pixels: for dilations 4 / 8 / 16 every
 // tap of a quad is one aligned 128-bit load (a shifted quad is entirely inside or outside the row because x0, W and d are multiples of
 // 4; row / column padding = out-of-range offsets of a bounded buffer resource), dilations 1 and 2 take the quad plus two edge pairs per
-// row; NCO x 4 accumulators per quad (v_pk_fma_f32 over pixel pairs), weights wave-uniform (s_load), one dilation per wave.  A lane
+// row; NCO x 4 accumulators per quad, weights wave-uniform (s_load), one dilation per wave.  A lane
 // that owned ONE quad (msq_kernel, earlier in round 3) loaded 9 pieces per channel and used none twice (the taps of a dilated window do
 // not overlap): bound by the number of tap loads going through L1 (profiles/r3_notes.md).  Here a lane owns R quads in rows y0, y0 + d, ..., y0 + (R - 1) d of one column block:
 // the rows y0 - d .. y0 + R d serve all of them -- 3 (R + 2) piece loads per channel for R quads instead of 9 R (R = 4: half,

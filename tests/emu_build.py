@@ -51,4 +51,5 @@ def lane_probe_make():
     """tests/emu/liblane_probe.so: one wave runs one real cross-lane instruction (gfx950 code object; hipcc cross-compiles it
     without a GPU)."""
     so, src = os.path.join(EMU, "liblane_probe.so"), os.path.join(EMU, "lane_probe.hip")
-    return _stamped(so, [src], ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O2", "-shared", "-fPIC", "-o", so, src])
+    return _stamped(so, [src], ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O2", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+                              "-shared", "-fPIC", "-o", so, src])

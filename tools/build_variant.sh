@@ -11,7 +11,7 @@ mkdir -p "$ROOT/gpurun_variants" /tmp/csn_obj
 python3 -c "import sys; sys.path.insert(0, '$ROOT'); from sod100k_amd import _native; _native.build()"
 cd "$ROOT/sod100k_amd/csrc"
 SRCS=$(python3 -c "import sys; sys.path.insert(0, '$ROOT'); from sod100k_amd import _native; print(' '.join(_native.SOURCES))")
-CC="/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-result"
+CC="/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops"
 objs=""
 for s in $SRCS; do
   if [[ ",$files," == *",$s,"* ]]; then
