@@ -37,7 +37,7 @@
 extern "C" {
 #endif
 
-#define CSN_ABI_VERSION 3   /* 2 (round 4): csn_profile_bracket_us, options 8-10; 3 (round 5): csn_build_sources_sha16, CSN_OPT_FUSE_ILB live again */
+#define CSN_ABI_VERSION 4   /* 2: csn_profile_bracket_us, options 8-10; 3: csn_build_sources_sha16, CSN_OPT_FUSE_ILB live again; 4: the training operators beside the plan */
 #define CSN_MAX_BRANCH 3
 #define CSN_NDIL 5
 
@@ -210,6 +210,76 @@ int csn_backward(csn_plan* plan, const float* x, const float* dy, void* workspac
 int csn_bce_with_logits(const float* y, const float* t, float* dy, int64_t n, double* loss, void* stream);
 int csn_adam_step(float* p, const float* g, float* m, float* v, const float* wd, int64_t n, float lr, float beta1,
                   float beta2, float eps, int32_t step, void* stream);
+
+/* ---- training operators beside the plan: 8-bit checkpoints of activations, layer norm, product gradients -----------------
+ * Free operators like csn_bce_with_logits: no plan, the caller owns every buffer, all launches go to `stream` (of the device that
+ * is current), no allocation, no synchronisation; they may be captured into a hipGraph.  Empty tensors are valid (their gradients
+ * are zero).  Sums, statistics and gradients are float (double across blocks) and every reduction has a fixed order.
+ *
+ * Layouts.  CSN_LAYOUT_PLANAR: [outer][channels][inner], the framework's planar maps, one token per pixel.
+ * CSN_LAYOUT_ROWS: [outer][channels], one token per row, inner = 1.  Inputs may be slices of wider tensors: element (o, c, p) lies
+ * at o * outer_stride + c * channel_stride + p (planar), o * outer_stride + c (rows; channel_stride is ignored); strides count
+ * elements and may be zero (broadcast).  Outputs are dense, weights and their gradients float.
+ *
+ * 8-bit checkpoint of a tensor (CSN_Q8_INT8 / CSN_Q8_E4M3): the elements of a plane (planar) or of a row (rows) in blocks of 32,
+ * the last block of each short; one byte of exponent s per block, one byte of code per element:
+ *     s = 127 + the smallest integer e >= -95 for which the block's largest finite |x| 2^-e rounds to at most 127 / 448,
+ *     code = x 2^-e rounded to the nearest integer (two's complement) / to the nearest OCP e4m3 number, ties to even,
+ *     value = code 2^(s - 127).
+ * The power of two makes both directions free of rounding but for the code's own: |value - x| is at most half a step of the code
+ * grid, and every value is exactly a bfloat16 number (what the product gradient's matrix instructions take).  Infinities, NaN and
+ * magnitudes from 1.9921875 x 2^127 (int8) / beyond 1.8125 x 2^127 (e4m3) on, which would round to 2^128, have one code (int8 -128,
+ * e4m3 0x7f) that unpacks to NaN; they do not touch the rest of their block ("finite" above leaves them out).  Codes are dense
+ * [rows][cols], exponents [rows][ceil(cols / 32)], a row being a plane or a row of tokens. */
+enum csn_dtype { CSN_F32 = 0, CSN_BF16 = 1 };
+enum csn_layout { CSN_LAYOUT_PLANAR = 0, CSN_LAYOUT_ROWS = 1 };
+enum csn_q8_format { CSN_Q8_INT8 = 0, CSN_Q8_E4M3 = 1 };
+#define CSN_Q8_BLOCK 32
+
+/* Element (o, r, c) of the input lies at o * outer_stride + r * row_stride + c; the checkpoint has outer * rows rows. */
+int csn_q8_pack(const void* x, int32_t dtype, int64_t outer, int64_t rows, int64_t cols, int64_t outer_stride,
+                int64_t row_stride, int32_t format, uint8_t* codes, uint8_t* exponents, void* stream);
+/* Dense values of a checkpoint of `rows` rows. */
+int csn_q8_unpack(const uint8_t* codes, const uint8_t* exponents, int32_t format, int64_t rows, int64_t cols, void* y,
+                  int32_t dtype, void* stream);
+
+typedef struct csn_norm_desc {
+  int32_t layout;   /* csn_layout */
+  int32_t dtype;    /* csn_dtype of x, y, dy and dx */
+  int64_t outer, channels, inner;
+  float eps;        /* > 0 */
+  int32_t format;   /* csn_q8_format of the checkpoint, where one is written or read */
+} csn_norm_desc;
+
+/* Layer norm over the channels of every token:  y = (x - mean) * rstd * weight + bias,  rstd = (var + eps)^(-1/2), var biased.
+ * weight / bias may be null (1 / 0); mean, rstd ([outer][inner]) may be null (inference).  codes / exponents, both or neither:
+ * the 8-bit checkpoint of x, written in the same pass. */
+int csn_layer_norm_forward(const csn_norm_desc* d, const void* x, int64_t x_outer_stride, int64_t x_channel_stride,
+                           const float* weight, const float* bias, void* y, float* mean, float* rstd, uint8_t* codes,
+                           uint8_t* exponents, void* stream);
+/* Gradients of a layer norm: dx (dense), dweight and dbias ([channels], WRITTEN; null = not wanted).  The input of the forward is
+ * given as x (with its strides) or as its checkpoint (codes, exponents; x null).  `workspace` (csn_layer_norm_workspace_bytes,
+ * any content) holds the partial weight gradients; one workspace per call in flight. */
+size_t csn_layer_norm_workspace_bytes(const csn_norm_desc* d);
+int csn_layer_norm_backward(const csn_norm_desc* d, const void* dy, int64_t dy_outer_stride, int64_t dy_channel_stride,
+                            const void* x, int64_t x_outer_stride, int64_t x_channel_stride, const uint8_t* codes,
+                            const uint8_t* exponents, const float* mean, const float* rstd, const float* weight, void* dx,
+                            float* dweight, float* dbias, void* workspace, size_t workspace_bytes, void* stream);
+
+typedef struct csn_product_desc {
+  int32_t layout, dtype, format;    /* dtype: of dy; format: of the input's checkpoint */
+  int32_t reserved;                 /* 0 */
+  int64_t outer, inner;             /* tokens = outer * inner */
+  int64_t cin, cout;
+} csn_product_desc;
+
+/* Weight and bias gradient of y[t] = W x[t] + b (a 1x1 convolution over planar maps, a linear layer over rows) from the checkpoint
+ * of x:  dweight[o][i] = sum_t dy[t][o] value(x[t][i]),  dbias[o] = sum_t dy[t][o]  (WRITTEN; dbias may be null).  bfloat16 dy
+ * and the values are multiplied exactly on the matrix cores, float dy as three bfloat16 parts (all 24 bits). */
+size_t csn_product_weight_grad_workspace_bytes(const csn_product_desc* d);
+int csn_product_weight_grad(const csn_product_desc* d, const void* dy, int64_t dy_outer_stride, int64_t dy_channel_stride,
+                            const uint8_t* codes, const uint8_t* exponents, float* dweight, float* dbias, void* workspace,
+                            size_t workspace_bytes, void* stream);
 
 /* The steps either side of csn_forward in the inference caller (CSNet/test.py), on the device:
  * csn_normalize_nchw: float H x W x 3 images in [0,1] (already at the network size) -> ImageNet-normalised NCHW

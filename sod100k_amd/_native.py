@@ -16,9 +16,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 # SOD100K_HIP_LIB: developer override (A/B builds of the same sources, e.g. the knock-out variants of profiles/r1_notes.md)
 LIB_PATH = os.environ.get("SOD100K_HIP_LIB") or os.path.join(CSRC, "libcsnet_hip.so")
-SOURCES = ("csn_plan.hip", "k_misc.hip", "k_goct_pw.hip", "k_ms.hip", "k_train.hip", "k_wgrad.hip", "k_wgrad_c3.hip", "k_wgrad_bf.hip", "k_goct_c3.hip", "k_csf.hip", "k_pw4.hip", "k_c3q.hip", "k_pwq.hip", "k_ilb.hip", "k_head.hip")
+SOURCES = ("csn_plan.hip", "k_misc.hip", "k_goct_pw.hip", "k_ms.hip", "k_train.hip", "k_wgrad.hip", "k_wgrad_c3.hip", "k_wgrad_bf.hip", "k_goct_c3.hip", "k_csf.hip", "k_pw4.hip", "k_c3q.hip", "k_pwq.hip", "k_ilb.hip", "k_head.hip",
+           "k_q8.hip", "k_norm.hip", "k_q8_wgrad.hip")
 
-ABI_VERSION = 3       # include/csnet_hip.h CSN_ABI_VERSION: checked BEFORE the entry points are bound (a stale .so lacks the new ones)
+ABI_VERSION = 4       # include/csnet_hip.h CSN_ABI_VERSION: checked BEFORE the entry points are bound (a stale .so lacks the new ones)
 
 
 def sources_sha16() -> str:
@@ -97,6 +98,24 @@ class TrainActInfo(C.Structure):
     _fields_ = [("act_offset_bytes", C.c_int64), ("z_offset_bytes", C.c_int64), ("grad_offset_bytes", C.c_int64 * 2),
                 ("x16_offset_bytes", C.c_int64), ("n_consumers", C.c_int32), ("bf16", C.c_int32),
                 ("dz_offset_bytes", C.c_int64)]
+
+
+DTYPE_F32, DTYPE_BF16 = 0, 1
+LAYOUT_PLANAR, LAYOUT_ROWS = 0, 1
+Q8_INT8, Q8_E4M3 = 0, 1
+Q8_BLOCK = 32
+
+
+class NormDesc(C.Structure):
+    """include/csnet_hip.h: csn_norm_desc."""
+    _fields_ = [("layout", C.c_int32), ("dtype", C.c_int32), ("outer", C.c_int64), ("channels", C.c_int64),
+                ("inner", C.c_int64), ("eps", C.c_float), ("format", C.c_int32)]
+
+
+class ProductDesc(C.Structure):
+    """include/csnet_hip.h: csn_product_desc."""
+    _fields_ = [("layout", C.c_int32), ("dtype", C.c_int32), ("format", C.c_int32), ("reserved", C.c_int32),
+                ("outer", C.c_int64), ("inner", C.c_int64), ("cin", C.c_int64), ("cout", C.c_int64)]
 
 
 class CsfGnOff(C.Structure):
@@ -287,6 +306,21 @@ def bind(lib: C.CDLL) -> C.CDLL:
     lib.csn_stream_copy.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]
     lib.csn_sal_hist.restype = C.c_int
     lib.csn_sal_hist.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]
+    p, i32, i64 = C.c_void_p, C.c_int32, C.c_int64
+    lib.csn_q8_pack.restype = C.c_int
+    lib.csn_q8_pack.argtypes = [p, i32, i64, i64, i64, i64, i64, i32, p, p, p]
+    lib.csn_q8_unpack.restype = C.c_int
+    lib.csn_q8_unpack.argtypes = [p, p, i32, i64, i64, p, i32, p]
+    lib.csn_layer_norm_forward.restype = C.c_int
+    lib.csn_layer_norm_forward.argtypes = [C.POINTER(NormDesc), p, i64, i64] + [p] * 8
+    lib.csn_layer_norm_workspace_bytes.restype = C.c_size_t
+    lib.csn_layer_norm_workspace_bytes.argtypes = [C.POINTER(NormDesc)]
+    lib.csn_layer_norm_backward.restype = C.c_int
+    lib.csn_layer_norm_backward.argtypes = [C.POINTER(NormDesc), p, i64, i64, p, i64, i64] + [p] * 9 + [C.c_size_t, p]
+    lib.csn_product_weight_grad_workspace_bytes.restype = C.c_size_t
+    lib.csn_product_weight_grad_workspace_bytes.argtypes = [C.POINTER(ProductDesc)]
+    lib.csn_product_weight_grad.restype = C.c_int
+    lib.csn_product_weight_grad.argtypes = [C.POINTER(ProductDesc), p, i64, i64] + [p] * 5 + [C.c_size_t, p]
     lib.csn_forward_profile.restype = C.c_int
     lib.csn_forward_profile.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                         C.c_int32, C.POINTER(C.c_float)]
@@ -328,7 +362,9 @@ EXPORTS: Sequence[str] = (
     "csn_forward", "csn_forward_train", "csn_plan_enable_training", "csn_backward", "csn_bce_with_logits",
            "csn_adam_step", "csn_val_mae", "csn_saliency_u8", "csn_normalize_nchw", "csn_resize_normalize_nchw", "csn_saliency_resize_u8", "csn_resize_bilinear", "csn_sal_hist", "csn_stream_copy", "csn_forward_profile", "csn_profile_num_kernels", "csn_profile_bracket_us", "csn_profile_kernel", "csn_unit_kernel_name", "csn_unit_algorithmic_bytes",
     "csf_head_create", "csf_head_destroy", "csf_head_workspace_bytes", "csf_head_refresh_params", "csf_head_forward",
-    "csf_head_stage_info", "csf_head_macs", "csf_bn_act", "csn_build_sources_sha16")
+    "csf_head_stage_info", "csf_head_macs", "csf_bn_act", "csn_build_sources_sha16",
+    "csn_q8_pack", "csn_q8_unpack", "csn_layer_norm_forward", "csn_layer_norm_workspace_bytes", "csn_layer_norm_backward",
+    "csn_product_weight_grad_workspace_bytes", "csn_product_weight_grad")
 
 _lib: Optional[C.CDLL] = None
 

@@ -14,6 +14,7 @@
 
 #include "../../include/csnet_hip.h"
 #include "csn_kernels.h"
+#include "train_ops.h"
 
 namespace {
 
@@ -2479,4 +2480,5 @@ int64_t csn_unit_algorithmic_bytes(const csn_plan* P, int32_t u) {
 
 }  // extern "C"
 
+#include "csn_train_ops.inl" // layer norm, 8-bit checkpoints, product gradients
 #include "csf_head.inl"      // CSF+Res2Net decoder head (include/csf_hip.h)

@@ -4,15 +4,15 @@
 //
 // The depthwise kernels are bound by vector-instruction issue, not by bytes (profiles/r4_notes.md: 83-85 % VALU utilisation; round 5's
 // issue_probe2 confirms every instruction pays its own slot).  Round 4's loop spent ~13 vector instructions per output pixel and unit:
-// nine taps as packed FMAs (4.5), BN as its own packed FMA (0.5), PReLU as multiply + compare + select (2.5), pair-building moves,
+// nine taps as paired FMAs (4.5), BN as its own paired FMA (0.5), PReLU as multiply + compare + select (2.5), pair-building moves,
 // per-element masks.  This core spends 4.5 + 1.5:
 //   * the BatchNorm scale is folded into the nine weights when the parameters are packed (w' = 100 w gamma / sqrt(var + eps),
-//     CSN_PREP_DWREC) and the shift is the accumulator's initial value: the nine packed FMAs ARE conv + BN;
+//     CSN_PREP_DWREC) and the shift is the accumulator's initial value: the nine paired FMAs ARE conv + BN;
 //   * PReLU(y) = max(y, alpha y) for alpha <= 1 and min(y, alpha y) for alpha > 1 = v_med3_f32(y, alpha y, +-inf): one packed
 //     multiply per pair and one median per value, no compare / select through VCC, any alpha;
-//   * a row of the 3-row window is kept as the FIVE overlapping pairs (v0,v1) .. (v4,v5) a packed FMA can take as an operand;
+//   * a row of the 3-row window is kept as the FIVE overlapping pairs (v0,v1) .. (v4,v5) a paired FMA can take as an operand;
 //     from LDS they are loaded as pairs (ds_read2_b32 delivers any two dwords into a register pair: no moves at all);
-//   * the two pair chains of a row's four outputs are interleaved, so no packed FMA waits for its predecessor.
+//   * the two pair chains of a row's four outputs are interleaved, so no paired FMA waits for its predecessor.
 #pragma once
 #include "csn_device.h"
 

@@ -1,0 +1,61 @@
+// train_ops.h -- argument blocks and launchers of the training operators beside the plan (k_q8.hip, k_norm.hip, k_q8_wgrad.hip).
+// Launchers return a hipError_t (0 = fine) or a negative number where no kernel takes the arguments.
+#pragma once
+#include <stdint.h>
+#include <stddef.h>
+
+struct Q8PackArgs {
+  const void* x;
+  uint8_t* codes;
+  uint8_t* exps;
+  int64_t outer, rows, cols, so, sr;   // element (o, r, c) at o * so + r * sr + c
+  int64_t nblk;                        // blocks of a row
+};
+struct Q8UnpackArgs {
+  const uint8_t* codes;
+  const uint8_t* exps;
+  void* y;
+  int64_t rows, cols, nblk;
+};
+int csn_launch_q8_pack(const Q8PackArgs& a, int a16, int fmt, void* stream);
+int csn_launch_q8_unpack(const Q8UnpackArgs& a, int a16, int fmt, void* stream);
+
+struct NormArgs {
+  const void* x;            // null: the checkpoint below is the input (backward)
+  const void* dy;
+  const uint8_t* codes_in;
+  const uint8_t* exps_in;
+  void* y;                  // forward: y, backward: dx
+  uint8_t* codes;           // forward: checkpoint of x (or null)
+  uint8_t* exps;
+  const float* weight;
+  const float* bias;
+  float* mean;
+  float* rstd;
+  float* dweight;
+  float* dbias;
+  float* partial;           // backward: [slabs][2][channels]
+  int64_t outer, C, inner;
+  int64_t x_so, x_sc, dy_so, dy_sc;
+  int64_t nblk;             // checkpoint blocks of a plane / row
+  float eps;
+  int32_t slabs;
+};
+int csn_launch_norm_fwd(const NormArgs& a, int rows, int a16, int fmt, void* stream);
+int csn_launch_norm_bwd(const NormArgs& a, int rows, int a16, int fmt, void* stream);
+int64_t csn_norm_partial_floats(int rows, int a16, int64_t outer, int64_t C, int64_t inner);
+
+struct Q8WgradArgs {
+  const void* dy;
+  const uint8_t* codes;
+  const uint8_t* exps;
+  float* dweight;
+  float* dbias;
+  float* partial;           // [slabs][cout][cin + 1]
+  int64_t outer, inner, cin, cout;
+  int64_t dy_so, dy_sc;
+  int64_t nblk;             // checkpoint blocks of a plane / row
+  int32_t slabs;
+};
+int csn_launch_q8_wgrad(const Q8WgradArgs& a, int rows, int a16, int fmt, void* stream);
+int64_t csn_q8_wgrad_partial_floats(int rows, int a16, int64_t outer, int64_t inner, int64_t cin, int64_t cout);

@@ -1,0 +1,366 @@
+"""Training operators beside the plan: layer norm, 8-bit checkpoints of activations, product gradients.
+
+Free operators of ``include/csnet_hip.h`` on torch tensors.  Like the functions of ``engine.py`` each takes the bound library
+first; PyTorch supplies device memory and the current stream, all arithmetic of the kernels happens in libcsnet_hip.so.  float32
+and bfloat16 tensors; weights, statistics and their gradients are float32.  A ``dim`` argument names the channel axis: ``1`` for
+planar maps ``[B, C, ...]`` (the framework's layout), ``-1`` for rows of tokens ``[..., C]``.
+
+``layer_norm`` and ``product`` at the end of the file are the differentiable forms.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes as C
+from typing import NamedTuple, Optional, Tuple, Union
+
+import torch
+
+from . import _native as N
+from .engine import _stream_of
+
+_DTYPES = {torch.float32: N.DTYPE_F32, torch.bfloat16: N.DTYPE_BF16}
+_FORMATS = {"int8": N.Q8_INT8, "e4m3": N.Q8_E4M3}
+
+
+class Q8(NamedTuple):
+    """8-bit checkpoint of a tensor: ``codes`` (uint8, the tensor's shape) and ``scales``, one power-of-two exponent byte per 32
+    elements of the axes from ``start_dim`` on, which count as one (``2`` for planar maps, ``-1`` for rows)."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    format: str
+    start_dim: int
+
+
+def _format(fmt: str) -> int:
+    if fmt not in _FORMATS:
+        raise ValueError(f"unknown checkpoint format {fmt!r} (one of {sorted(_FORMATS)})")
+    return _FORMATS[fmt]
+
+
+def _dtype(t: torch.Tensor, what: str) -> int:
+    if t.dtype not in _DTYPES:
+        raise TypeError(f"{what}: float32 or bfloat16 expected, got {t.dtype}")
+    return _DTYPES[t.dtype]
+
+
+def _same_device(lib: C.CDLL, *tensors: Optional[torch.Tensor]) -> torch.device:
+    """The tensors' one device.  The product library works on ROCm tensors only (no CPU fallback)."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if dev is not None and t.device != dev:
+            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+        dev = t.device
+    if (dev.type == "cuda") != (lib is N._lib):
+        raise RuntimeError(f"this library does not work on {dev.type} tensors (the HIP path is ROCm only: there is no CPU fallback)")
+    return dev
+
+
+def _on(dev: torch.device):
+    """Launches go to the device that is current: make it the tensors' own."""
+    if dev.type == "cuda" and torch.cuda.current_device() != dev.index:
+        return torch.cuda.device(dev)
+    return contextlib.nullcontext()
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _channel_axis(dim: int, ndim: int) -> bool:
+    """True for rows (the channels are the last axis), False for planar maps (axis 1 of at least three)."""
+    if not -ndim <= dim < ndim:
+        raise ValueError(f"dim {dim} out of range for {ndim} axes")
+    if dim % ndim == ndim - 1:
+        return True
+    if dim % ndim == 1:
+        return False
+    raise ValueError("the channel axis is the last one (rows) or axis 1 (planar maps)")
+
+
+def _view(x: torch.Tensor, rows: bool) -> Tuple[torch.Tensor, int, int]:
+    """(tensor, outer stride, channel stride) of x as [tokens][C] or [B][C][pixels] with consecutive innermost elements; slices of
+    wider tensors are taken as they lie, anything else is copied."""
+    v = x.reshape(-1, x.shape[-1]) if rows else x.flatten(2)
+    if v.shape[-1] > 1 and v.stride(-1) != 1:
+        v = v.contiguous()
+    so = v.stride(0) if v.shape[0] > 1 else 0
+    return v, so, (0 if rows or v.shape[1] <= 1 else v.stride(1))
+
+
+def _blocks(cols: int) -> int:
+    return -(-cols // N.Q8_BLOCK)
+
+
+def _scales_shape(shape, start_dim: int) -> Tuple[int, ...]:
+    cols = 1
+    for s in shape[start_dim:]:
+        cols *= s
+    return tuple(shape[:start_dim]) + (_blocks(cols),)
+
+
+def _check_q8(q: Q8) -> int:
+    f = _format(q.format)
+    if q.codes.dtype != torch.uint8 or q.scales.dtype != torch.uint8:
+        raise TypeError("codes and scales of a checkpoint are uint8")
+    if not q.codes.is_contiguous() or not q.scales.is_contiguous():
+        raise ValueError("codes and scales of a checkpoint are contiguous")
+    if q.start_dim not in (2, -1) or q.codes.dim() < (3 if q.start_dim == 2 else 1):
+        raise ValueError("a checkpoint's blocks run along the last axis (start_dim -1) or over a map's pixels (start_dim 2)")
+    if tuple(q.scales.shape) != _scales_shape(q.codes.shape, q.start_dim):
+        raise ValueError(f"scales of shape {tuple(q.scales.shape)}, expected {_scales_shape(q.codes.shape, q.start_dim)}")
+    return f
+
+
+def _q8_rows(q: Q8) -> Tuple[int, int]:
+    cols = 1
+    for s in q.codes.shape[q.start_dim:]:
+        cols *= s
+    return (q.codes.numel() // cols if cols else 0), cols
+
+
+def q8_pack(lib: C.CDLL, x: torch.Tensor, format: str = "int8", start_dim: int = -1) -> Q8:
+    """8-bit checkpoint of ``x`` ("int8" or "e4m3").  The axes from ``start_dim`` on form the rows that are cut into blocks of 32:
+    ``2`` for planar maps [B, C, ...], ``-1`` for rows [..., C]."""
+    f, dt = _format(format), _dtype(x, "q8_pack")
+    dev = _same_device(lib, x)
+    if start_dim not in (2, -1) or x.dim() < (3 if start_dim == 2 else 1):
+        raise ValueError("start_dim is -1 (the last axis) or 2 (the pixels of planar maps [B, C, ...])")
+    rows = start_dim == -1
+    codes = torch.empty(x.shape, dtype=torch.uint8, device=dev)
+    scales = torch.empty(_scales_shape(x.shape, start_dim), dtype=torch.uint8, device=dev)
+    if x.numel():
+        v, so, sc = _view(x, rows)
+        o, r, c, s0, s1 = (1, v.shape[0], v.shape[1], 0, so) if rows else (v.shape[0], v.shape[1], v.shape[2], so, sc)
+        with _on(dev):
+            N.check(lib, lib.csn_q8_pack(v.data_ptr(), dt, o, r, c, s0, s1, f, codes.data_ptr(), scales.data_ptr(), _stream_of(x)),
+                    "csn_q8_pack")
+    return Q8(codes, scales, format, start_dim)
+
+
+def q8_unpack(lib: C.CDLL, q: Q8, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values of a checkpoint as a dense float32 or bfloat16 tensor (both hold them exactly)."""
+    f = _check_q8(q)
+    dev = _same_device(lib, q.codes, q.scales)
+    y = torch.empty(q.codes.shape, dtype=dtype, device=dev)
+    dt = _dtype(y, "q8_unpack")
+    if y.numel():
+        rows, cols = _q8_rows(q)
+        with _on(dev):
+            N.check(lib, lib.csn_q8_unpack(q.codes.data_ptr(), q.scales.data_ptr(), f, rows, cols, y.data_ptr(), dt, _stream_of(y)),
+                    "csn_q8_unpack")
+    return y
+
+
+def _param(t: Optional[torch.Tensor], channels: int, what: str) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    if t.dtype != torch.float32:
+        raise TypeError(f"{what}: float32 expected, got {t.dtype}")
+    if tuple(t.shape) != (channels,):
+        raise ValueError(f"{what}: shape ({channels},) expected, got {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def _norm_desc(rows: bool, dt: int, shape, eps: float, fmt: int) -> N.NormDesc:
+    d = N.NormDesc()
+    d.layout, d.dtype, d.eps, d.format = (N.LAYOUT_ROWS if rows else N.LAYOUT_PLANAR), dt, float(eps), fmt
+    d.outer, d.channels, d.inner = 1, (shape[-1] if rows else shape[1]), 1
+    for s in (shape[:-1] if rows else shape[:1]):
+        d.outer *= s
+    for s in (() if rows else shape[2:]):
+        d.inner *= s
+    return d
+
+
+def layer_norm_forward(lib: C.CDLL, x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                       dim: int = -1, eps: float = 1e-5, checkpoint: Optional[str] = None
+                       ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, Optional[Q8]]:
+    """``(y, mean, rstd, checkpoint)`` of the layer norm over axis ``dim``: ``y`` dense in x's dtype, the statistics float32 with
+    x's shape without that axis, and, with ``checkpoint`` "int8" / "e4m3", the 8-bit checkpoint of x written in the same pass
+    (else None)."""
+    dt = _dtype(x, "layer_norm")
+    rows = _channel_axis(dim, x.dim())
+    ch = x.shape[-1] if rows else x.shape[1]
+    weight, bias = _param(weight, ch, "weight"), _param(bias, ch, "bias")
+    dev = _same_device(lib, x, weight, bias)
+    fmt = _format(checkpoint) if checkpoint is not None else 0
+    d = _norm_desc(rows, dt, x.shape, eps, fmt)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    sshape = x.shape[:-1] if rows else x.shape[:1] + x.shape[2:]
+    mean = torch.empty(sshape, dtype=torch.float32, device=dev)
+    rstd = torch.empty(sshape, dtype=torch.float32, device=dev)
+    q = None
+    if checkpoint is not None:
+        start = -1 if rows else 2
+        q = Q8(torch.empty(x.shape, dtype=torch.uint8, device=dev),
+               torch.empty(_scales_shape(x.shape, start), dtype=torch.uint8, device=dev), checkpoint, start)
+    v, so, sc = _view(x, rows) if x.numel() else (x, 0, 0)
+    with _on(dev):
+        N.check(lib, lib.csn_layer_norm_forward(C.byref(d), v.data_ptr(), so, sc, _ptr(weight), _ptr(bias), y.data_ptr(),
+                                                mean.data_ptr(), rstd.data_ptr(), _ptr(q.codes) if q and x.numel() else None,
+                                                _ptr(q.scales) if q and x.numel() else None, _stream_of(x)), "csn_layer_norm_forward")
+    return y, mean, rstd, q
+
+
+def layer_norm_backward(lib: C.CDLL, dy: torch.Tensor, x: Union[torch.Tensor, Q8], mean: torch.Tensor, rstd: torch.Tensor,
+                        weight: Optional[torch.Tensor] = None, dim: int = -1
+                        ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(dx, dweight, dbias)`` of a layer norm from its input ``x`` -- the tensor or its checkpoint -- and the statistics of the
+    forward.  ``dx`` is dense in dy's dtype, the parameter gradients float32."""
+    dt = _dtype(dy, "layer_norm")
+    rows = _channel_axis(dim, dy.dim())
+    ch = dy.shape[-1] if rows else dy.shape[1]
+    weight = _param(weight, ch, "weight")
+    q = x if isinstance(x, Q8) else None
+    fmt = _check_q8(q) if q is not None else 0
+    src = q.codes if q is not None else x
+    if src.shape != dy.shape:
+        raise ValueError(f"dy of shape {tuple(dy.shape)}, the input has {tuple(src.shape)}")
+    if q is None and x.dtype != dy.dtype:
+        raise TypeError(f"dy is {dy.dtype}, the input {x.dtype}")
+    if q is not None and q.start_dim != (-1 if rows else 2):
+        raise ValueError("the checkpoint was packed for the other layout")
+    sshape = tuple(dy.shape[:-1] if rows else dy.shape[:1] + dy.shape[2:])
+    for t, what in ((mean, "mean"), (rstd, "rstd")):
+        if t.dtype != torch.float32 or tuple(t.shape) != sshape:
+            raise ValueError(f"{what}: float32 of shape {sshape} expected, got {t.dtype} {tuple(t.shape)}")
+    mean, rstd = mean.contiguous(), rstd.contiguous()
+    dev = _same_device(lib, dy, src, q.scales if q is not None else None, mean, rstd, weight)
+    d = _norm_desc(rows, dt, dy.shape, 1.0, fmt)
+    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev)
+    dweight = torch.empty(ch, dtype=torch.float32, device=dev)
+    dbias = torch.empty(ch, dtype=torch.float32, device=dev)
+    nbytes = int(lib.csn_layer_norm_workspace_bytes(C.byref(d)))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    vd, dso, dsc = _view(dy, rows) if dy.numel() else (dy, 0, 0)
+    vx, so, sc = _view(x, rows) if q is None and dy.numel() else (None, 0, 0)
+    with _on(dev):
+        N.check(lib, lib.csn_layer_norm_backward(C.byref(d), vd.data_ptr(), dso, dsc, _ptr(vx), so, sc,
+                                                 _ptr(q.codes) if q is not None and dy.numel() else None,
+                                                 _ptr(q.scales) if q is not None and dy.numel() else None, mean.data_ptr(),
+                                                 rstd.data_ptr(), _ptr(weight), dx.data_ptr(), dweight.data_ptr(),
+                                                 dbias.data_ptr(), _ptr(ws), nbytes, _stream_of(dy)), "csn_layer_norm_backward")
+    return dx, dweight, dbias
+
+
+def product_weight_grad(lib: C.CDLL, dy: torch.Tensor, q: Q8, dim: int = -1) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(dweight [Cout, Cin], dbias [Cout])``, float32, of a 1x1 convolution (``dim=1``) or linear layer (``dim=-1``) from the
+    gradient of its output and the checkpoint of its input."""
+    dt = _dtype(dy, "product_weight_grad")
+    fmt = _check_q8(q)
+    rows = _channel_axis(dim, dy.dim())
+    if q.start_dim != (-1 if rows else 2):
+        raise ValueError("the checkpoint was packed for the other layout")
+    xs, ds = tuple(q.codes.shape), tuple(dy.shape)
+    if (xs[:-1] != ds[:-1]) if rows else (len(xs) != len(ds) or xs[:1] + xs[2:] != ds[:1] + ds[2:]):
+        raise ValueError(f"dy of shape {ds} does not belong to an input of shape {xs}")
+    dev = _same_device(lib, dy, q.codes, q.scales)
+    nd = _norm_desc(rows, dt, ds, 1.0, fmt)
+    d = N.ProductDesc()
+    d.layout, d.dtype, d.format, d.outer, d.inner = nd.layout, dt, fmt, nd.outer, nd.inner
+    d.cin, d.cout = (xs[-1], ds[-1]) if rows else (xs[1], ds[1])
+    dweight = torch.empty((d.cout, d.cin), dtype=torch.float32, device=dev)
+    dbias = torch.empty(d.cout, dtype=torch.float32, device=dev)
+    nbytes = int(lib.csn_product_weight_grad_workspace_bytes(C.byref(d)))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    v, so, sc = _view(dy, rows) if dy.numel() else (dy, 0, 0)
+    with _on(dev):
+        N.check(lib, lib.csn_product_weight_grad(C.byref(d), v.data_ptr(), so, sc, q.codes.data_ptr(), q.scales.data_ptr(),
+                                                 dweight.data_ptr(), dbias.data_ptr(), _ptr(ws), nbytes, _stream_of(dy)),
+                "csn_product_weight_grad")
+    return dweight, dbias
+
+
+# ---- differentiable forms -------------------------------------------------------------------------------------------------
+def _refuse_capture() -> None:
+    """Autograd inside a stream capture depends on what other graphs of the same leaves live on (their accumulation nodes keep the
+    stream they were made on, and the engine's wait for it breaks the capture): the raw forms above are for captures."""
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("layer_norm / product with gradients inside a stream capture: capture the *_forward / *_backward / "
+                           "*_weight_grad functions instead")
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, lib, x, weight, bias, dim, eps, checkpoint):
+        if any(ctx.needs_input_grad):
+            _refuse_capture()
+        y, mean, rstd, q = layer_norm_forward(lib, x, weight, bias, dim=dim, eps=eps, checkpoint=checkpoint)
+        ctx.lib, ctx.dim = lib, dim
+        if q is None:
+            ctx.save_for_backward(mean, rstd, weight, x)
+            ctx.q = None
+        else:
+            ctx.save_for_backward(mean, rstd, weight, q.codes, q.scales)
+            ctx.q = (q.format, q.start_dim)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        _refuse_capture()
+        mean, rstd, weight, *src = ctx.saved_tensors
+        x = src[0] if ctx.q is None else Q8(src[0], src[1], *ctx.q)
+        dx, dw, db = layer_norm_backward(ctx.lib, dy, x, mean, rstd, weight, dim=ctx.dim)
+        need = ctx.needs_input_grad
+        return None, dx if need[1] else None, dw if need[2] else None, db if need[3] else None, None, None, None
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, dim: int = -1,
+               eps: float = 1e-5, checkpoint: Optional[str] = None, lib: Optional[C.CDLL] = None) -> torch.Tensor:
+    """Differentiable layer norm over axis ``dim``.  ``checkpoint`` ("int8" / "e4m3") keeps x for the backward in 8 bits instead of
+    the tensor itself: the gradients are then those of the checkpoint's values."""
+    return _LayerNormFn.apply(lib or N.load(), x, weight, bias, dim, eps, checkpoint)
+
+
+def _product(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], rows: bool) -> torch.Tensor:
+    """The forward product itself: one library matrix product in x's dtype."""
+    w = weight.to(x.dtype)
+    b = None if bias is None else bias.to(x.dtype)
+    if rows:
+        return torch.nn.functional.linear(x, w, b)
+    y = torch.matmul(w, x.flatten(2).contiguous())
+    if b is not None:
+        y += b.view(1, -1, 1)
+    return y.view(x.shape[:1] + (w.shape[0],) + x.shape[2:])
+
+
+class _ProductFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, lib, x, weight, bias, dim, checkpoint):
+        if any(ctx.needs_input_grad):
+            _refuse_capture()
+        rows = _channel_axis(dim, x.dim())
+        y = _product(x, weight, bias, rows)
+        ctx.lib, ctx.dim, ctx.rows = lib, dim, rows
+        q = q8_pack(lib, x, checkpoint, start_dim=-1 if rows else 2)
+        ctx.q = (q.format, q.start_dim)
+        ctx.save_for_backward(weight, q.codes, q.scales)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        _refuse_capture()
+        weight, codes, scales = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx = dw = db = None
+        if need[1]:
+            dx = _product(dy, weight.t().contiguous(), None, ctx.rows)
+        if need[2] or need[3]:
+            dw, db = product_weight_grad(ctx.lib, dy, Q8(codes, scales, *ctx.q), dim=ctx.dim)
+        return None, dx, dw if need[2] else None, db if need[3] else None, None, None
+
+
+def product(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, dim: int = -1, checkpoint: str = "int8",
+            lib: Optional[C.CDLL] = None) -> torch.Tensor:
+    """Differentiable 1x1 convolution over planar maps (``dim=1``) or linear layer over rows (``dim=-1``), weight [Cout, Cin], that
+    keeps its input for the weight gradient as an 8-bit checkpoint.  The forward and the input gradient are exact library products
+    in x's dtype; only the weight gradient sees the checkpoint's values."""
+    ch = x.shape[-1] if _channel_axis(dim, x.dim()) else x.shape[1]
+    if weight.dim() != 2 or weight.shape[1] != ch or weight.dtype != torch.float32:
+        raise ValueError(f"weight: float32 of shape (Cout, {ch}) expected, got {weight.dtype} {tuple(weight.shape)}")
+    bias = _param(bias, weight.shape[0], "bias")
+    return _ProductFn.apply(lib or N.load(), x, weight, bias, dim, checkpoint)

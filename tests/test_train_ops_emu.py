@@ -1,0 +1,106 @@
+"""Training operators beside the plan on the CPU emulation of their kernels (lane-exact mode: the device paths), and the refusals of
+their Python and C entry points."""
+import ctypes
+import os
+
+import pytest
+import torch
+
+import train_ops_cases as K
+from sod100k_amd import _native as N, train_ops as T
+
+
+@pytest.fixture(scope="module")
+def lib(emu_lanes_lib):
+    return emu_lanes_lib[0]
+
+
+@pytest.mark.parametrize("fmt", K.FORMATS)
+@pytest.mark.parametrize("dtype", K.DTYPES)
+def test_emu_pack(lib, fmt, dtype):
+    for i, (shape, start) in enumerate(K.PACK_SHAPES):
+        K.check_pack(lib, K.activations(shape, dtype, i, rows=start == -1), fmt, start)
+    K.check_pack(lib, K.block_edge_values(dtype), fmt, -1)
+
+
+@pytest.mark.parametrize("fmt", K.FORMATS)
+def test_emu_every_code(lib, fmt):
+    q, want = K.every_code_once(fmt)
+    for dtype in K.DTYPES:
+        v = T.q8_unpack(lib, q, dtype)
+        assert K.same(v.double(), want)
+
+
+@pytest.mark.parametrize("dtype", K.DTYPES)
+@pytest.mark.parametrize("shape,dim", K.NORM_SHAPES)
+def test_emu_norm(lib, shape, dim, dtype):
+    rows = dim == -1
+    x, dy = K.activations(shape, dtype, 1, rows=rows), K.gradient(shape, dtype, 1)
+    w, b = K.params(shape[dim], 1)
+    y, mean, rstd, _ = K.check_norm_forward(lib, x, w, b, dim)
+    K.check_norm_forward(lib, x, None, None, dim)
+    K.check_norm_backward(lib, dy, x, mean, rstd, w, dim)
+    K.check_norm_backward(lib, dy, x, mean, rstd, None, dim)
+    for fmt in K.FORMATS:
+        y2, m2, r2, q = K.check_norm_forward(lib, x, w, b, dim, checkpoint=fmt)
+        assert torch.equal(y, y2) and torch.equal(mean, m2) and torch.equal(rstd, r2)
+        K.check_norm_backward(lib, dy, x, mean, rstd, w, dim, q=q)
+
+
+@pytest.mark.parametrize("fmt", K.FORMATS)
+@pytest.mark.parametrize("dtype", K.DTYPES)
+def test_emu_product_gradient(lib, dtype, fmt):
+    for i, (dims, cin, cout, dim) in enumerate(K.PRODUCT_SHAPES):
+        x, dy = K.product_tensors(dims, cin, cout, dim, dtype, i)
+        K.check_product(lib, dy, x, fmt, dim)
+
+
+@pytest.mark.parametrize("dtype", K.DTYPES)
+def test_emu_slices_and_strides(lib, dtype):
+    K.check_slices(lib, "cpu", dtype)
+
+
+def test_emu_empty(lib):
+    K.check_empty(lib, "cpu")
+
+
+@pytest.mark.parametrize("dtype", K.DTYPES)
+def test_emu_bad_tokens_stay_alone(lib, dtype):
+    K.check_bad_tokens_stay_alone(lib, "cpu", dtype)
+
+
+def test_emu_constant_tokens_and_far_means(lib):
+    K.check_constant_and_far(lib, "cpu")
+
+
+def test_emu_determinism(lib):
+    K.check_determinism(lib, "cpu")
+
+
+def test_emu_gradients_against_differences(lib):
+    K.check_against_differences(lib, "cpu")
+
+
+@pytest.mark.parametrize("dtype", K.DTYPES)
+def test_emu_norm_and_product_together(lib, dtype):
+    K.check_block_of_operators(lib, "cpu", dtype)
+
+
+def test_refusals(lib):
+    K.check_refusals(lib, "cpu")
+    K.check_refusals_of_the_abi(lib)
+
+
+def test_refusals_of_the_product_library():
+    """The same refusals from the library that runs on the GPU: they are host code and follow no pointer."""
+    if not os.path.exists(N.LIB_PATH):
+        pytest.skip("libcsnet_hip.so not built")
+    K.check_refusals_of_the_abi(N.bind(ctypes.CDLL(N.LIB_PATH)))
+
+
+def test_no_cpu_fallback(lib, monkeypatch):
+    monkeypatch.setattr(N, "_lib", lib)      # the library that load() returned takes ROCm tensors only
+    with pytest.raises(RuntimeError, match="ROCm"):
+        T.layer_norm_forward(lib, torch.zeros(2, 4))
+    with pytest.raises(RuntimeError, match="ROCm"):
+        T.q8_pack(lib, torch.zeros(2, 4))
