@@ -7,6 +7,7 @@
 #include "csn_reduce.h"
 #include "q8_core.h"
 #include "train_ops.h"
+#include "vec_io.h"
 
 // channel c of token (o, p), from x or from its checkpoint
 template <typename AT, int FMT, bool ROWS>
@@ -20,7 +21,7 @@ __device__ __forceinline__ float norm_dy(const NormArgs& a, int64_t o, int64_t p
   return act_ld(reinterpret_cast<const AT*>(a.dy) + o * a.dy_so + (ROWS ? c : c * a.dy_sc + p));
 }
 
-// one block per token
+// ---- simple forms, for tokens of more channels than the register forms below hold: one block per token / per channel
 template <typename AT, bool ROWS>
 __global__ __launch_bounds__(CSN_BLOCK) void norm_fwd_kernel(NormArgs a) {
   CSN_DYN_SMEM(double, sm);
@@ -70,7 +71,6 @@ __global__ __launch_bounds__(CSN_BLOCK) void norm_bwd_kernel(NormArgs a) {
   }
 }
 
-// one block per channel
 template <typename AT, int FMT, bool ROWS>
 __global__ __launch_bounds__(CSN_BLOCK) void norm_dw_kernel(NormArgs a) {
   CSN_DYN_SMEM(double, sm);
@@ -91,7 +91,559 @@ __global__ __launch_bounds__(CSN_BLOCK) void norm_dw_kernel(NormArgs a) {
   }
 }
 
+
 static unsigned norm_grid(int64_t items) { return (unsigned)(items < 16384 ? items : 16384); }
+
+#ifndef CSN_EMU_SEQ
+// ---- the fast forms: a token's channels stay in registers -----------------------------------------------------------------
+enum { NORM_X = -1 };   // input of the backward: x itself (else a checkpoint format); forward: no checkpoint is written
+
+// sums over G lanes (a power of two): a butterfly inside the wave, then the block's waves in order through LDS (two buffers of
+// [N][16] floats in turn: one barrier per sum)
+template <int G, int N>
+__device__ __forceinline__ void norm_sum(float (&v)[N], float* sm, int& turn) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (G >= 64) v[i] += csn_lane_xor_f32<32>(v[i]);
+    if (G >= 32) v[i] += csn_lane_xor_f32<16>(v[i]);
+    if (G >= 16) v[i] += csn_lane_xor_f32<8>(v[i]);
+    if (G >= 8) v[i] += csn_lane_xor_f32<4>(v[i]);
+    v[i] += csn_lane_xor_f32<2>(v[i]);
+    v[i] += csn_lane_xor_f32<1>(v[i]);
+  }
+  if (G > 64) {
+    float* b = sm + turn * (N * 16);
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int i = 0; i < N; ++i) b[i * 16 + (threadIdx.x >> 6)] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < G / 64; ++w) s += b[i * 16 + w];
+      v[i] = s;
+    }
+  }
+}
+
+template <int G> struct NormRowsBlock { static constexpr int T = G > CSN_BLOCK ? G : CSN_BLOCK; };
+
+// Rows of tokens: G lanes per token, NV pieces of E elements (16 bytes) per lane.  A block walks tokens, its weights in registers.
+template <typename AT, int G, int NV, int CK>
+__global__ __launch_bounds__(NormRowsBlock<G>::T) void norm_rows_fwd_kernel(NormArgs a) {
+  constexpr int E = VecIo<AT>::E, T = NormRowsBlock<G>::T, R = T / G;
+  CSN_DYN_SMEM(float, sm);
+  const int l = threadIdx.x % G, C = (int)a.C;
+  const float inv_c = 1.f / (float)C;
+  const bool wide = C >= E;
+  float w[NV][E], b[NV][E];
+  int n[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int c0 = E * (l + G * v);
+    n[v] = C - c0;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      w[v][j] = a.weight && j < n[v] ? a.weight[c0 + j] : 1.f;
+      b[v][j] = a.bias && j < n[v] ? a.bias[c0 + j] : 0.f;
+    }
+  }
+  int turn = 0;
+  for (int64_t t = (int64_t)blockIdx.x * R + threadIdx.x / G; t < a.outer; t += (int64_t)gridDim.x * R) {
+    const AT* x = reinterpret_cast<const AT*>(a.x) + t * a.x_so;
+    VecIo<AT> r[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) vec_load(r[v], x + E * (l + G * v), n[v], wide);
+    float s[1] = {0.f};
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      float f[E];
+      vec_end(r[v], n[v], wide);
+      r[v].get(f);
+#pragma unroll
+      for (int j = 0; j < E; ++j) s[0] += f[j];
+    }
+    norm_sum<G, 1>(s, sm, turn);
+    const float mean = s[0] / (float)C;   // (divided: equal channels have no variance at all)
+    s[0] = 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      float f[E];
+      r[v].pin();
+      r[v].get(f);
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float d = j < n[v] ? f[j] - mean : 0.f;
+        s[0] = fmaf(d, d, s[0]);
+      }
+    }
+    norm_sum<G, 1>(s, sm, turn);
+    const float rstd = 1.f / sqrtf(fmaf(s[0], inv_c, a.eps));
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c0 = E * (l + G * v);
+      float f[E], y[E];
+      r[v].pin();
+      r[v].get(f);
+#pragma unroll
+      for (int j = 0; j < E; ++j) y[j] = fmaf((f[j] - mean) * rstd, w[v][j], b[v][j]);
+      VecIo<AT>::store(reinterpret_cast<AT*>(a.y) + t * C + c0, y, n[v]);
+      if (CK >= 0) {
+        const unsigned e = q8_block_exponent<CK, E>(f);
+        unsigned c[E / 4];
+        q8_encode_vec<CK, E>(f, q8_inv_scale(e), c);
+        code_store<E>(a.codes + t * C + c0, c, n[v]);
+        if ((l & (32 / E - 1)) == 0 && n[v] > 0) a.exps[t * a.nblk + (c0 >> 5)] = (uint8_t)e;
+      }
+    }
+    if (l == 0) {
+      if (a.mean) a.mean[t] = mean;
+      if (a.rstd) a.rstd[t] = rstd;
+    }
+  }
+}
+
+// one piece of the backward's input, the tensor or its checkpoint
+template <typename AT, int SRC> struct NormIn {
+  static constexpr int E = VecIo<AT>::E;
+  CodeIo<E> c;
+  float scale;
+  __device__ __forceinline__ void end(int n, bool wide) { code_end<E>(c, n, wide); }
+  __device__ __forceinline__ void pin() { c.pin(); }
+  __device__ __forceinline__ void get(float (&f)[E]) const { q8_decode_vec<SRC, E>(c.w, scale, f); }
+};
+template <typename AT> struct NormIn<AT, NORM_X> {
+  static constexpr int E = VecIo<AT>::E;
+  VecIo<AT> v;
+  __device__ __forceinline__ void end(int n, bool wide) { vec_end(v, n, wide); }
+  __device__ __forceinline__ void pin() { v.pin(); }
+  __device__ __forceinline__ void get(float (&f)[E]) const { v.get(f); }
+};
+
+template <typename AT, int G, int NV, int SRC>
+__global__ __launch_bounds__(NormRowsBlock<G>::T) void norm_rows_bwd_kernel(NormArgs a) {
+  constexpr int E = VecIo<AT>::E, T = NormRowsBlock<G>::T, R = T / G;
+  CSN_DYN_SMEM(float, sm);
+  const int l = threadIdx.x % G, C = (int)a.C;
+  const float inv_c = 1.f / (float)C;
+  const bool wide = C >= E;
+  float w[NV][E], dw[NV][E], db[NV][E];
+  int n[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int c0 = E * (l + G * v);
+    n[v] = C - c0;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      w[v][j] = a.weight && j < n[v] ? a.weight[c0 + j] : 1.f;
+      dw[v][j] = db[v][j] = 0.f;
+    }
+  }
+  int turn = 0;
+  for (int64_t t = (int64_t)blockIdx.x * R + threadIdx.x / G; t < a.outer; t += (int64_t)gridDim.x * R) {
+    const AT* dy = reinterpret_cast<const AT*>(a.dy) + t * a.dy_so;
+    NormIn<AT, SRC> rx[NV];
+    VecIo<AT> rd[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c0 = E * (l + G * v);
+      if constexpr (SRC == NORM_X) {
+        vec_load(rx[v].v, reinterpret_cast<const AT*>(a.x) + t * a.x_so + c0, n[v], wide);
+      } else {
+        code_load<E>(rx[v].c, a.codes_in + t * C + c0, n[v], wide);
+        rx[v].scale = n[v] > 0 ? q8_scale(a.exps_in[t * a.nblk + (c0 >> 5)]) : 1.f;
+      }
+      vec_load(rd[v], dy + c0, n[v], wide);
+    }
+    const float mean = a.mean[t], rstd = a.rstd[t];
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      float f[E], d[E];
+      rx[v].end(n[v], wide);
+      vec_end(rd[v], n[v], wide);
+      rx[v].get(f);
+      rd[v].get(d);
+#pragma unroll
+      for (int j = 0; j < E; ++j) {   // (past the end: d = 0)
+        const float xh = (f[j] - mean) * rstd, g = d[j] * w[v][j];
+        s[0] += g;
+        s[1] = j < n[v] ? fmaf(g, xh, s[1]) : s[1];
+        dw[v][j] = fmaf(d[j], xh, dw[v][j]);
+        db[v][j] += d[j];
+      }
+    }
+    norm_sum<G, 2>(s, sm, turn);
+    const float c1 = s[0] * inv_c, c2 = s[1] * inv_c;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      float f[E], d[E], o[E];
+      rx[v].pin();
+      rd[v].pin();
+      rx[v].get(f);
+      rd[v].get(d);
+#pragma unroll
+      for (int j = 0; j < E; ++j) o[j] = rstd * (fmaf(d[j], w[v][j], -c1) - (f[j] - mean) * rstd * c2);
+      VecIo<AT>::store(reinterpret_cast<AT*>(a.y) + t * C + E * (l + G * v), o, n[v]);
+    }
+  }
+  if (!a.partial) return;
+  // the block's R tokens at a time share columns: added in order, one slab per block
+  float* p = a.partial + (int64_t)blockIdx.x * 2 * C;
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c0 = E * (l + G * v);
+      float o[E];
+#pragma unroll
+      for (int j = 0; j < E; ++j) o[j] = q ? db[v][j] : dw[v][j];
+      if (R > 1) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < E; ++j) sm[threadIdx.x * E + j] = o[j];
+        __syncthreads();
+        if (threadIdx.x < G) {
+#pragma unroll 1
+          for (int k = 1; k < R; ++k)
+#pragma unroll
+            for (int j = 0; j < E; ++j) o[j] += sm[(k * G + threadIdx.x) * E + j];
+        }
+      }
+      if (threadIdx.x < G)
+#pragma unroll
+        for (int h = 0; h < E; h += 4) {
+          const float four[4] = {o[h], o[h + 1], o[h + 2], o[h + 3]};
+          VecIo<float>::store(p + q * C + c0 + h, four, n[v] - h);
+        }
+    }
+}
+
+// Planar maps: PX lanes along the pixels (E consecutive pixels of a channel, 16 bytes, per lane), T / PX groups of lanes over the
+// channels, NC channels per lane in registers.  Sums over a pixel's channels: butterfly over the groups of a wave, then the waves in
+// order through LDS (two buffers of [waves][N][PX * E] floats in turn).
+template <int T, int PX, int E, int N>
+__device__ __forceinline__ void norm_planar_sum(float (&v)[N][E], float* sm, int& turn) {
+  constexpr int W = T / 64, TP = PX * E;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      v[i][j] += csn_lane_xor_f32<32>(v[i][j]);
+      if (PX <= 16) v[i][j] += csn_lane_xor_f32<16>(v[i][j]);
+      if (PX <= 8) v[i][j] += csn_lane_xor_f32<8>(v[i][j]);
+      if (PX <= 4) v[i][j] += csn_lane_xor_f32<4>(v[i][j]);
+      if (PX <= 2) v[i][j] += csn_lane_xor_f32<2>(v[i][j]);
+    }
+  float* b = sm + turn * (W * N * TP);
+  turn ^= 1;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, px = lane % PX;
+  if (lane < PX)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int j = 0; j < E; ++j) b[(wave * N + i) * TP + px * E + j] = v[i][j];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < E; ++j) v[i][j] = 0.f;
+#pragma unroll 2   // (all at once would hold T / 4 registers)
+  for (int k = 0; k < W; ++k)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[i][j] += b[(k * N + i) * TP + px * E + j];
+}
+
+// (image, pixel tile) items of a persistent launch.  Addresses are a uniform base -- image, tile, group of channels k -- plus one
+// 32-bit offset per lane that all of its channels share.
+template <typename AT, int T, int PX, int NC, int CK>
+__global__ __launch_bounds__(T) void norm_planar_fwd_kernel(NormArgs a) {
+  constexpr int E = VecIo<AT>::E, CG = T / PX, TP = PX * E;
+  CSN_DYN_SMEM(float, sm);
+  const int px = threadIdx.x % PX, cg = threadIdx.x / PX, C = (int)a.C, P = (int)a.inner;
+  const float inv_c = 1.f / (float)C;
+  const bool wide = P >= E;
+  float w[NC], b[NC];
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
+    const int c = cg + CG * k;
+    w[k] = a.weight && c < C ? a.weight[c] : 1.f;
+    b[k] = a.bias && c < C ? a.bias[c] : 0.f;
+  }
+  const unsigned xoff = (unsigned)cg * (unsigned)a.x_sc + px * E, yoff = (unsigned)cg * (unsigned)P + px * E;
+  int turn = 0;
+  for (int it = blockIdx.x; it < a.items; it += gridDim.x) {
+    const int o = it / a.tiles, t0 = (it - o * a.tiles) * TP;
+    const int n = P - t0 - px * E;
+    const AT* x = reinterpret_cast<const AT*>(a.x) + o * a.x_so + t0;
+    VecIo<AT> r[NC];
+#pragma unroll
+    for (int k = 0; k < NC; ++k) vec_load(r[k], x + (int64_t)(CG * k) * a.x_sc + xoff, cg + CG * k < C ? n : 0, wide);
+    float s[1][E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) s[0][j] = 0.f;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      float f[E];
+      vec_end(r[k], n, wide);
+      r[k].get(f);
+#pragma unroll
+      for (int j = 0; j < E; ++j) s[0][j] += f[j];
+    }
+    norm_planar_sum<T, PX, E, 1>(s, sm, turn);
+    float mean[E], rstd[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) { mean[j] = s[0][j] / (float)C; s[0][j] = 0.f; }   // (divided: as above)
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      float f[E];
+      r[k].pin();
+      r[k].get(f);
+      if (cg + CG * k < C)
+#pragma unroll
+        for (int j = 0; j < E; ++j) s[0][j] = fmaf(f[j] - mean[j], f[j] - mean[j], s[0][j]);
+    }
+    norm_planar_sum<T, PX, E, 1>(s, sm, turn);
+#pragma unroll
+    for (int j = 0; j < E; ++j) rstd[j] = 1.f / sqrtf(fmaf(s[0][j], inv_c, a.eps));
+    const int64_t row0 = (int64_t)o * C;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int c = cg + CG * k;
+      float f[E], y[E];
+      r[k].pin();
+      r[k].get(f);
+#pragma unroll
+      for (int j = 0; j < E; ++j) y[j] = fmaf((f[j] - mean[j]) * rstd[j], w[k], b[k]);
+      const int64_t base = (row0 + CG * k) * P + t0;
+      if (c < C) VecIo<AT>::store(reinterpret_cast<AT*>(a.y) + base + yoff, y, n);
+      if (CK >= 0) {
+        const unsigned e = q8_block_exponent<CK, E>(f);
+        unsigned q[E / 4];
+        q8_encode_vec<CK, E>(f, q8_inv_scale(e), q);
+        if (c < C) {
+          code_store<E>(a.codes + base + yoff, q, n);
+          if ((px & (32 / E - 1)) == 0 && n > 0) a.exps[(row0 + c) * a.nblk + ((t0 + px * E) >> 5)] = (uint8_t)e;
+        }
+      }
+    }
+    if (cg == 0) {
+      const int64_t st = (int64_t)o * P + t0 + px * E;
+      if (a.mean)
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (j < n) a.mean[st + j] = mean[j];
+      if (a.rstd)
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (j < n) a.rstd[st + j] = rstd[j];
+    }
+  }
+}
+
+template <typename AT, int T, int PX, int NC, int SRC>
+__global__ __launch_bounds__(T) void norm_planar_bwd_kernel(NormArgs a) {
+  constexpr int E = VecIo<AT>::E, CG = T / PX, TP = PX * E;
+  CSN_DYN_SMEM(float, sm);
+  const int px = threadIdx.x % PX, cg = threadIdx.x / PX, C = (int)a.C, P = (int)a.inner;
+  const float inv_c = 1.f / (float)C;
+  const bool wide = P >= E;
+  float w[NC], dw[NC], db[NC];
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
+    w[k] = a.weight && cg + CG * k < C ? a.weight[cg + CG * k] : 1.f;
+    dw[k] = db[k] = 0.f;
+  }
+  const unsigned xoff = (unsigned)cg * (unsigned)a.x_sc + px * E, doff = (unsigned)cg * (unsigned)a.dy_sc + px * E;
+  const unsigned yoff = (unsigned)cg * (unsigned)P + px * E;
+  int turn = 0;
+  for (int it = blockIdx.x; it < a.items; it += gridDim.x) {
+    const int o = it / a.tiles, t0 = (it - o * a.tiles) * TP;
+    const int n = P - t0 - px * E;
+    const int64_t row0 = (int64_t)o * C;
+    const AT* x = reinterpret_cast<const AT*>(a.x) + o * a.x_so + t0;
+    const AT* dy = reinterpret_cast<const AT*>(a.dy) + o * a.dy_so + t0;
+    NormIn<AT, SRC> rx[NC];
+    VecIo<AT> rd[NC];
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int m = cg + CG * k < C ? n : 0;
+      if constexpr (SRC == NORM_X) {
+        vec_load(rx[k].v, x + (int64_t)(CG * k) * a.x_sc + xoff, m, wide);
+      } else {
+        code_load<E>(rx[k].c, a.codes_in + (row0 + CG * k) * P + t0 + yoff, m, wide);
+        rx[k].scale = m > 0 ? q8_scale(a.exps_in[(row0 + cg + CG * k) * a.nblk + ((t0 + px * E) >> 5)]) : 1.f;
+      }
+      vec_load(rd[k], dy + (int64_t)(CG * k) * a.dy_sc + doff, m, wide);
+    }
+    float mean[E], rstd[E], s[2][E];
+    const int64_t st = (int64_t)o * P + t0 + px * E;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      mean[j] = j < n ? a.mean[st + j] : 0.f;
+      rstd[j] = j < n ? a.rstd[st + j] : 0.f;
+      s[0][j] = s[1][j] = 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      float f[E], d[E];
+      rx[k].end(n, wide);
+      vec_end(rd[k], n, wide);
+      rx[k].get(f);
+      rd[k].get(d);
+#pragma unroll
+      for (int j = 0; j < E; ++j) {   // (channels and pixels past the end: f = d = 0)
+        const float xh = (f[j] - mean[j]) * rstd[j], g = d[j] * w[k];
+        s[0][j] += g;
+        s[1][j] = fmaf(g, xh, s[1][j]);
+        dw[k] = fmaf(d[j], xh, dw[k]);
+        db[k] += d[j];
+      }
+    }
+    norm_planar_sum<T, PX, E, 2>(s, sm, turn);
+#pragma unroll
+    for (int j = 0; j < E; ++j) { s[0][j] *= inv_c; s[1][j] *= inv_c * rstd[j]; }
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      float f[E], d[E], y[E];
+      rx[k].pin();
+      rd[k].pin();
+      rx[k].get(f);
+      rd[k].get(d);
+#pragma unroll
+      for (int j = 0; j < E; ++j) y[j] = rstd[j] * (fmaf(d[j], w[k], -s[0][j]) - (f[j] - mean[j]) * s[1][j]);
+      if (cg + CG * k < C) VecIo<AT>::store(reinterpret_cast<AT*>(a.y) + (row0 + CG * k) * P + t0 + yoff, y, n);
+    }
+  }
+  if (!a.partial) return;
+  float* p = a.partial + (int64_t)blockIdx.x * 2 * C;
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
+    float u = dw[k], v = db[k];
+    if (PX >= 16) { u += csn_lane_xor_f32<8>(u); v += csn_lane_xor_f32<8>(v); }
+    if (PX >= 8) { u += csn_lane_xor_f32<4>(u); v += csn_lane_xor_f32<4>(v); }
+    if (PX >= 4) { u += csn_lane_xor_f32<2>(u); v += csn_lane_xor_f32<2>(v); }
+    u += csn_lane_xor_f32<1>(u); v += csn_lane_xor_f32<1>(v);
+    const int c = cg + CG * k;
+    if (px == 0 && c < C) { p[c] = u; p[C + c] = v; }
+  }
+}
+
+// dweight / dbias: the blocks' slabs in order, 64 columns per block, wave w adds slabs w, w + 16, ...
+__global__ __launch_bounds__(1024) void norm_reduce_kernel(NormArgs a) {
+  CSN_DYN_SMEM(double, sd);   // [16][64]
+  const int64_t n = 2 * a.C, e = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const int w = threadIdx.x >> 6;
+  double v = 0.0;
+  if (e < n) {
+#pragma unroll 4
+    for (int s = w; s < a.slabs; s += 16) v += a.partial[(int64_t)s * n + e];
+  }
+  sd[w * 64 + (threadIdx.x & 63)] = v;
+  __syncthreads();
+  if (w == 0 && e < n) {
+    for (int q = 1; q < 16; ++q) v += sd[q * 64 + (threadIdx.x & 63)];
+    float* out = e < a.C ? a.dweight : a.dbias;
+    if (out) out[e < a.C ? e : e - a.C] = (float)v;
+  }
+}
+
+// blocks of a persistent launch: the chip's 256 CUs full of waves
+static int64_t norm_blocks(int threads) { return 256 * (int64_t)(2048 / threads); }
+
+// The register forms: which one takes a case, what its grid is.  slabs = 0: none.
+struct NormPlan { int G, NV; int T, PX, NC; int64_t slabs, tiles, items; };
+static NormPlan norm_plan(int rows, int a16, bool bwd, int64_t outer, int64_t C, int64_t inner, int64_t x_sc, int64_t dy_sc) {
+  NormPlan p{};
+  if (outer * inner == 0) return p;
+  if (rows) {   // NV counts pieces of 8 elements
+    if (C > 16384) return p;
+    p.G = C <= 64 ? 8 : C <= 128 ? 16 : C <= 256 ? 32 : C <= 1024 ? 64 : C <= 4096 ? 256 : 1024;
+    p.NV = C <= (int64_t)p.G * 8 ? 1 : 2;
+    p.T = std::max(p.G, CSN_BLOCK);
+    const int r = p.T / p.G;
+    p.slabs = std::min(norm_blocks(p.T), (outer + r - 1) / r);
+    return p;
+  }
+  if (C > 4096) return p;
+  // the forward holds 16 bytes per channel and lane, the backward 32 and two sums
+  p.T = C <= 128 ? 256 : C <= 256 ? 512 : 1024;
+  p.PX = C <= 64 ? 16 : C <= 512 ? 8 : bwd ? (C <= 1024 ? 4 : 2) : (C <= 2048 ? 8 : 4);
+  const int cg = p.T / p.PX;
+  p.NC = C <= 4 * cg ? 4 : C <= 8 * cg ? 8 : 16;
+  const int64_t tile = (int64_t)p.PX * (a16 ? 8 : 4), lim = (int64_t)1 << 30;
+  p.tiles = (inner + tile - 1) / tile;
+  p.items = outer * p.tiles;
+  // 32-bit offsets of a lane and 32-bit item counts
+  if (inner > lim || p.items > lim || cg * std::max(inner, std::max(x_sc, dy_sc)) + tile > lim) { p.slabs = 0; return p; }
+  p.slabs = std::min(norm_blocks(p.T), p.items);
+  return p;
+}
+
+template <typename AT, int G, int NVB, int CK>
+static int norm_rows_go(const NormArgs& a, bool bwd, void* stream) {
+  constexpr int NV = NVB * (8 / VecIo<AT>::E), T = NormRowsBlock<G>::T;
+  const dim3 g((unsigned)a.slabs), b(T);
+  const size_t sm = std::max((size_t)64 * sizeof(float), T / G > 1 ? (size_t)T * VecIo<AT>::E * sizeof(float) : (size_t)0);
+  if (bwd) CSN_LAUNCH((norm_rows_bwd_kernel<AT, G, NV, CK>), g, b, sm, stream, a);
+  else CSN_LAUNCH((norm_rows_fwd_kernel<AT, G, NV, CK>), g, b, sm, stream, a);
+  return (int)hipGetLastError();
+}
+template <typename AT, int CK>
+static int norm_rows_run(const NormArgs& a, const NormPlan& p, bool bwd, void* stream) {
+  switch (p.G) {
+    case 8: return norm_rows_go<AT, 8, 1, CK>(a, bwd, stream);
+    case 16: return norm_rows_go<AT, 16, 1, CK>(a, bwd, stream);
+    case 32: return norm_rows_go<AT, 32, 1, CK>(a, bwd, stream);
+    case 64: return p.NV == 1 ? norm_rows_go<AT, 64, 1, CK>(a, bwd, stream) : norm_rows_go<AT, 64, 2, CK>(a, bwd, stream);
+    case 256: return p.NV == 1 ? norm_rows_go<AT, 256, 1, CK>(a, bwd, stream) : norm_rows_go<AT, 256, 2, CK>(a, bwd, stream);
+  }
+  return p.NV == 1 ? norm_rows_go<AT, 1024, 1, CK>(a, bwd, stream) : norm_rows_go<AT, 1024, 2, CK>(a, bwd, stream);
+}
+template <typename AT, int T, int PX, int NC, int CK>
+static int norm_planar_fwd_go(const NormArgs& a, void* stream) {
+  const size_t sm = (size_t)2 * (T / 64) * PX * VecIo<AT>::E * sizeof(float);
+  CSN_LAUNCH((norm_planar_fwd_kernel<AT, T, PX, NC, CK>), dim3((unsigned)a.slabs), dim3(T), sm, stream, a);
+  return (int)hipGetLastError();
+}
+template <typename AT, int T, int PX, int NC, int CK>
+static int norm_planar_bwd_go(const NormArgs& a, void* stream) {
+  const size_t sm = (size_t)2 * (T / 64) * 2 * PX * VecIo<AT>::E * sizeof(float);
+  CSN_LAUNCH((norm_planar_bwd_kernel<AT, T, PX, NC, CK>), dim3((unsigned)a.slabs), dim3(T), sm, stream, a);
+  return (int)hipGetLastError();
+}
+template <typename AT, int CK>
+static int norm_planar_run(const NormArgs& a, const NormPlan& p, bool bwd, void* stream) {
+  if (p.T == 256 && p.PX == 16) return bwd ? norm_planar_bwd_go<AT, 256, 16, 4, CK>(a, stream) : norm_planar_fwd_go<AT, 256, 16, 4, CK>(a, stream);
+  if (p.T == 256) return bwd ? norm_planar_bwd_go<AT, 256, 8, 4, CK>(a, stream) : norm_planar_fwd_go<AT, 256, 8, 4, CK>(a, stream);
+  if (p.T == 512) return bwd ? norm_planar_bwd_go<AT, 512, 8, 4, CK>(a, stream) : norm_planar_fwd_go<AT, 512, 8, 4, CK>(a, stream);
+  if (!bwd) {
+    if (p.NC == 4) return norm_planar_fwd_go<AT, 1024, 8, 4, CK>(a, stream);
+    if (p.NC == 8) return norm_planar_fwd_go<AT, 1024, 8, 8, CK>(a, stream);
+    return p.PX == 8 ? norm_planar_fwd_go<AT, 1024, 8, 16, CK>(a, stream) : norm_planar_fwd_go<AT, 1024, 4, 16, CK>(a, stream);
+  }
+  if (p.PX == 8) return norm_planar_bwd_go<AT, 1024, 8, 4, CK>(a, stream);
+  if (p.PX == 4) return norm_planar_bwd_go<AT, 1024, 4, 4, CK>(a, stream);
+  return p.NC == 4 ? norm_planar_bwd_go<AT, 1024, 2, 4, CK>(a, stream) : norm_planar_bwd_go<AT, 1024, 2, 8, CK>(a, stream);
+}
+template <int CK>
+static int norm_fast(const NormArgs& a, const NormPlan& p, int rows, int a16, bool bwd, void* stream) {
+  if (rows) return a16 ? norm_rows_run<csn_bf16, CK>(a, p, bwd, stream) : norm_rows_run<float, CK>(a, p, bwd, stream);
+  return a16 ? norm_planar_run<csn_bf16, CK>(a, p, bwd, stream) : norm_planar_run<float, CK>(a, p, bwd, stream);
+}
+static int norm_fast(NormArgs a, const NormPlan& p, int rows, int a16, int ck, bool bwd, void* stream) {
+  a.slabs = (int32_t)p.slabs; a.tiles = (int32_t)p.tiles; a.items = (int32_t)p.items;
+  if (ck == NORM_X) return norm_fast<NORM_X>(a, p, rows, a16, bwd, stream);
+  return ck == Q8_INT8 ? norm_fast<Q8_INT8>(a, p, rows, a16, bwd, stream) : norm_fast<Q8_E4M3>(a, p, rows, a16, bwd, stream);
+}
+#else
+struct NormPlan { int64_t slabs; };
+static NormPlan norm_plan(int, int, bool, int64_t, int64_t, int64_t, int64_t, int64_t) { return NormPlan{0}; }
+#endif  // CSN_EMU_SEQ
 
 template <typename AT, bool ROWS>
 static int norm_fwd(const NormArgs& a, void* stream) {
@@ -100,16 +652,23 @@ static int norm_fwd(const NormArgs& a, void* stream) {
   return (int)hipGetLastError();
 }
 
-int csn_launch_norm_fwd(const NormArgs& a, int rows, int a16, int fmt, void* stream) {
+int csn_launch_norm_fwd(const NormArgs& a0, int rows, int a16, int fmt, void* stream) {
+  NormArgs a = a0;
   if (a.outer * a.inner <= 0) return 0;
-  if (a.codes) {   // the checkpoint of x as a pass of its own
+  const NormPlan p = norm_plan(rows, a16, false, a.outer, a.C, a.inner, a.x_sc, 0);
+  // a lane's neighbours hold a whole block of 32 in every register form but the widest planar one in float
+  if (a.codes && (p.slabs == 0 || (!rows && !a16 && a.C > 2048))) {   // the checkpoint of x as a pass of its own
     Q8PackArgs q;
     q.x = a.x; q.codes = a.codes; q.exps = a.exps; q.nblk = a.nblk;
     q.outer = rows ? 1 : a.outer; q.rows = rows ? a.outer : a.C; q.cols = rows ? a.C : a.inner;
     q.so = rows ? 0 : a.x_so; q.sr = rows ? a.x_so : a.x_sc;
     const int e = csn_launch_q8_pack(q, a16, fmt, stream);
     if (e != 0) return e;
+    a.codes = nullptr;
   }
+#ifndef CSN_EMU_SEQ
+  if (p.slabs > 0) return norm_fast(a, p, rows, a16, a.codes ? fmt : NORM_X, false, stream);
+#endif
   if (rows) return a16 ? norm_fwd<csn_bf16, true>(a, stream) : norm_fwd<float, true>(a, stream);
   return a16 ? norm_fwd<csn_bf16, false>(a, stream) : norm_fwd<float, false>(a, stream);
 }
@@ -123,7 +682,19 @@ static int norm_bwd(const NormArgs& a, void* stream) {
   return (int)hipGetLastError();
 }
 
-int csn_launch_norm_bwd(const NormArgs& a, int rows, int a16, int fmt, void* stream) {
+int csn_launch_norm_bwd(const NormArgs& a0, int rows, int a16, int fmt, void* stream) {
+  NormArgs a = a0;
+  const NormPlan p = norm_plan(rows, a16, true, a.outer, a.C, a.inner, a.x_sc, a.dy_sc);
+#ifndef CSN_EMU_SEQ
+  if (p.slabs > 0) {
+    if (!a.dweight && !a.dbias) a.partial = nullptr;
+    const int e = norm_fast(a, p, rows, a16, a.x ? NORM_X : fmt, true, stream);
+    if (e != 0 || !a.partial) return e;
+    a.slabs = (int32_t)p.slabs;
+    CSN_LAUNCH(norm_reduce_kernel, dim3((unsigned)((2 * a.C + 63) / 64)), dim3(1024), 1024 * sizeof(double), stream, a);
+    return (int)hipGetLastError();
+  }
+#endif
   if (fmt == Q8_INT8) {
     if (rows) return a16 ? norm_bwd<csn_bf16, Q8_INT8, true>(a, stream) : norm_bwd<float, Q8_INT8, true>(a, stream);
     return a16 ? norm_bwd<csn_bf16, Q8_INT8, false>(a, stream) : norm_bwd<float, Q8_INT8, false>(a, stream);
@@ -132,4 +703,6 @@ int csn_launch_norm_bwd(const NormArgs& a, int rows, int a16, int fmt, void* str
   return a16 ? norm_bwd<csn_bf16, Q8_E4M3, false>(a, stream) : norm_bwd<float, Q8_E4M3, false>(a, stream);
 }
 
-int64_t csn_norm_partial_floats(int, int, int64_t, int64_t, int64_t) { return 0; }
+int64_t csn_norm_partial_floats(int rows, int a16, int64_t outer, int64_t C, int64_t inner) {
+  return norm_plan(rows, a16, true, outer, C, inner, 0, 0).slabs * 2 * C;   // (strides only ever lower the count)
+}

@@ -60,3 +60,30 @@ __device__ __forceinline__ float q8_decode(unsigned c, float scale) {
   if (FMT == Q8_INT8) return c == Q8_NAN_INT8 ? csn_bits_f(0x7fc00000u) : (float)(int)(signed char)c * scale;
   return q8_from_e4m3(c) * scale;
 }
+
+// E codes at once, packed in dwords
+template <int FMT, int E>
+__device__ __forceinline__ void q8_encode_vec(const float (&f)[E], float inv, unsigned (&w)[E / 4]) {
+#pragma unroll
+  for (int j = 0; j < E / 4; ++j)
+    w[j] = q8_encode<FMT>(f[4 * j], inv) | q8_encode<FMT>(f[4 * j + 1], inv) << 8 | q8_encode<FMT>(f[4 * j + 2], inv) << 16 |
+           q8_encode<FMT>(f[4 * j + 3], inv) << 24;
+}
+template <int FMT, int E>
+__device__ __forceinline__ void q8_decode_vec(const unsigned (&w)[E / 4], float scale, float (&f)[E]) {
+#pragma unroll
+  for (int j = 0; j < E; ++j) f[j] = q8_decode<FMT>((w[j >> 2] >> (8 * (j & 3))) & 0xffu, scale);
+}
+#ifndef CSN_EMU_SEQ
+// exponent of the block that the 32 / E neighbouring lanes hold together
+template <int FMT, int E>
+__device__ __forceinline__ unsigned q8_block_exponent(const float (&f)[E]) {
+  float m = 0.f;
+#pragma unroll
+  for (int j = 0; j < E; ++j) m = fmaxf(m, q8_mag<FMT>(f[j]));
+  m = fmaxf(m, csn_lane_xor_f32<1>(m));
+  m = fmaxf(m, csn_lane_xor_f32<2>(m));
+  if (E == 4) m = fmaxf(m, csn_lane_xor_f32<4>(m));
+  return q8_exponent<FMT>(m);
+}
+#endif

@@ -41,7 +41,9 @@ struct NormArgs {
   int64_t x_so, x_sc, dy_so, dy_sc;
   int64_t nblk;             // checkpoint blocks of a plane / row
   float eps;
-  int32_t slabs;
+  // set by the launcher
+  int32_t slabs;            // blocks of the register forms
+  int32_t tiles, items;     // planar: pixel tiles of an image, (image, tile) items
 };
 int csn_launch_norm_fwd(const NormArgs& a, int rows, int a16, int fmt, void* stream);
 int csn_launch_norm_bwd(const NormArgs& a, int rows, int a16, int fmt, void* stream);

@@ -223,7 +223,7 @@ def check_product(lib, dy, x, fmt, dim):
 # inside a block and a vector
 NORM_SHAPES = [((1, 1), -1), ((1, 2048), -1), ((7, 8), -1), ((5, 33), -1), ((130, 64), -1), ((3, 331), -1), ((2, 9, 80), -1), ((2, 5000), -1),
                ((1, 20000), -1), ((70, 1000), -1), ((1, 1, 1, 1), 1), ((2, 79, 5, 7), 1), ((1, 40, 28, 28), 1), ((3, 20, 1, 1), 1),
-               ((2, 8, 33), 1), ((1, 300, 6, 6), 1), ((2, 64, 16, 16), 1), ((1, 2, 100, 3), 1), ((1, 1100, 4, 8), 1), ((1, 64, 40, 40), 1)]
+               ((2, 8, 33), 1), ((1, 300, 6, 6), 1), ((2, 64, 16, 16), 1), ((1, 2, 100, 3), 1), ((1, 1100, 4, 8), 1), ((1, 64, 40, 40), 1), ((1, 3000, 5, 7), 1), ((1, 5000, 1, 3), 1), ((1, 33000), -1)]
 PACK_SHAPES = [((1,), -1), ((3, 31), -1), ((2, 32), -1), ((5, 33), -1), ((4, 64), -1), ((3, 7, 100), -1), ((2, 3, 5, 9), 2), ((1, 4, 8, 8), 2),
                ((2, 2, 1, 1), 2), ((3, 40, 14, 14), 2)]
 # (outer dims of x, cin, cout, dim)
