@@ -191,9 +191,8 @@ __global__ __launch_bounds__(NormRowsBlock<G>::T) void norm_rows_fwd_kernel(Norm
       for (int j = 0; j < E; ++j) y[j] = fmaf((f[j] - mean) * rstd, w[v][j], b[v][j]);
       VecIo<AT>::store(reinterpret_cast<AT*>(a.y) + t * C + c0, y, n[v]);
       if (CK >= 0) {
-        const unsigned e = q8_block_exponent<CK, E>(f);
         unsigned c[E / 4];
-        q8_encode_vec<CK, E>(f, q8_inv_scale(e), c);
+        const unsigned e = q8_pack_block<CK, E>(f, c);
         code_store<E>(a.codes + t * C + c0, c, n[v]);
         if ((l & (32 / E - 1)) == 0 && n[v] > 0) a.exps[t * a.nblk + (c0 >> 5)] = (uint8_t)e;
       }
@@ -422,9 +421,8 @@ __global__ __launch_bounds__(T) void norm_planar_fwd_kernel(NormArgs a) {
       const int64_t base = (row0 + CG * k) * P + t0;
       if (c < C) VecIo<AT>::store(reinterpret_cast<AT*>(a.y) + base + yoff, y, n);
       if (CK >= 0) {
-        const unsigned e = q8_block_exponent<CK, E>(f);
         unsigned q[E / 4];
-        q8_encode_vec<CK, E>(f, q8_inv_scale(e), q);
+        const unsigned e = q8_pack_block<CK, E>(f, q);
         if (c < C) {
           code_store<E>(a.codes + base + yoff, q, n);
           if ((px & (32 / E - 1)) == 0 && n > 0) a.exps[(row0 + c) * a.nblk + ((t0 + px * E) >> 5)] = (uint8_t)e;

@@ -34,7 +34,13 @@ __device__ __forceinline__ csn_u4 wg_u4(unsigned a, unsigned b, unsigned c, unsi
   return r;
 }
 // {the high halves of a and b}: two bfloat16 by truncation
-__device__ __forceinline__ unsigned wg_hi2(float a, float b) { return (csn_f_bits(a) >> 16) | (csn_f_bits(b) & 0xffff0000u); }
+__device__ __forceinline__ unsigned wg_hi2(float a, float b) {
+#ifdef CSN_CPU_EMU
+  return (csn_f_bits(a) >> 16) | (csn_f_bits(b) & 0xffff0000u);
+#else
+  return __builtin_amdgcn_perm(csn_f_bits(b), csn_f_bits(a), 0x07060302u);
+#endif
+}
 // one of the three parts of a float and what is left of it
 __device__ __forceinline__ float wg_cut(float& x) {
   const float h = csn_bits_f(csn_f_bits(x) & 0xffff0000u);
@@ -112,13 +118,6 @@ template <> struct WgY4<float> {
   }
   __device__ __forceinline__ float get(int j) const { return j == 0 ? a.x : j == 1 ? a.y : j == 2 ? a.z : a.w; }
 };
-
-// four codes as values
-template <int FMT>
-__device__ __forceinline__ void wg_decode4(unsigned w, float scale, float (&f)[4]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) f[j] = q8_decode<FMT>((w >> (8 * j)) & 0xffu, scale);
-}
 
 // n = 0 .. 4 codes from an address of any alignment
 __device__ __forceinline__ unsigned wg_codes(const uint8_t* p, int n) {
@@ -238,11 +237,11 @@ __global__ __launch_bounds__(CSN_BLOCK) void q8_wgrad_kernel(Q8WgradArgs a) {
 #pragma unroll
       for (int j = 0; j < TN / 32; ++j) {
         const float sc = q8_scale(rg.s[j]);
-        float f[4], g[4];
-        wg_decode4<FMT>(rg.x[j].x, sc, f);
-        wg_decode4<FMT>(rg.x[j].y, sc, g);
+        const unsigned w[2] = {rg.x[j].x, rg.x[j].y};
+        float f[8];
+        q8_decode_vec<FMT, 8>(w, sc, f);
         *reinterpret_cast<csn_u4*>(bx + wg_piece((tid >> 3) + 32 * j, tid & 7)) =
-            wg_u4(wg_hi2(f[0], f[1]), wg_hi2(f[2], f[3]), wg_hi2(g[0], g[1]), wg_hi2(g[2], g[3]));
+            wg_u4(wg_hi2(f[0], f[1]), wg_hi2(f[2], f[3]), wg_hi2(f[4], f[5]), wg_hi2(f[6], f[7]));
       }
     } else {
       constexpr int GY = TM / 4, GX = TN / 4;
@@ -268,7 +267,10 @@ __global__ __launch_bounds__(CSN_BLOCK) void q8_wgrad_kernel(Q8WgradArgs a) {
         const int c = 4 * (tid & (GX - 1)), k = tid / GX;
         float f[8][4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) wg_decode4<FMT>(rg.x[j], q8_scale(rg.s[j]), f[j]);
+        for (int j = 0; j < 8; ++j) {
+          const unsigned w[1] = {rg.x[j]};
+          q8_decode_vec<FMT, 4>(w, q8_scale(rg.s[j]), f[j]);
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           *reinterpret_cast<csn_u4*>(bx + wg_piece(c + q, k)) =

@@ -12,12 +12,14 @@ struct Q8PackArgs {
   uint8_t* exps;
   int64_t outer, rows, cols, so, sr;   // element (o, r, c) at o * so + r * sr + c
   int64_t nblk;                        // blocks of a row
+  int64_t nrows, per_row, items;       // (set by the launcher) rows, pieces of a row, pieces
 };
 struct Q8UnpackArgs {
   const uint8_t* codes;
   const uint8_t* exps;
   void* y;
   int64_t rows, cols, nblk;
+  int64_t per_row, items;              // (set by the launcher)
 };
 int csn_launch_q8_pack(const Q8PackArgs& a, int a16, int fmt, void* stream);
 int csn_launch_q8_unpack(const Q8UnpackArgs& a, int a16, int fmt, void* stream);

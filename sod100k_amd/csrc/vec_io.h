@@ -9,6 +9,7 @@
 
 struct __attribute__((packed, aligned(2))) csn_raw16_a2 { unsigned w[4]; };
 struct __attribute__((packed, aligned(4))) csn_raw16_a4 { unsigned w[4]; };
+struct __attribute__((packed, aligned(1))) csn_raw16_a1 { unsigned w[4]; };
 struct __attribute__((packed, aligned(1))) csn_raw8_a1 { unsigned w[2]; };
 struct __attribute__((packed, aligned(1))) csn_raw4_a1 { unsigned w[1]; };
 
