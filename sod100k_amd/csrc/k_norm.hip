@@ -128,6 +128,12 @@ __device__ __forceinline__ void norm_sum(float (&v)[N], float* sm, int& turn) {
   }
 }
 
+// where the block's sums of dy xh (q = 0) / of dy (q = 1) go: its slab, or the gradient itself where there is one block; null: not wanted
+__device__ __forceinline__ float* norm_slab(const NormArgs& a, int q) {
+  if (gridDim.x == 1) return q ? a.dbias : a.dweight;
+  return a.partial ? a.partial + ((int64_t)blockIdx.x * 2 + q) * a.C : nullptr;
+}
+
 template <int G> struct NormRowsBlock { static constexpr int T = G > CSN_BLOCK ? G : CSN_BLOCK; };
 
 // Rows of tokens: G lanes per token, NV pieces of E elements (16 bytes) per lane.  A block walks tokens, its weights in registers.
@@ -288,11 +294,11 @@ __global__ __launch_bounds__(NormRowsBlock<G>::T) void norm_rows_bwd_kernel(Norm
       VecIo<AT>::store(reinterpret_cast<AT*>(a.y) + t * C + E * (l + G * v), o, n[v]);
     }
   }
-  if (!a.partial) return;
-  // the block's R tokens at a time share columns: added in order, one slab per block
-  float* p = a.partial + (int64_t)blockIdx.x * 2 * C;
+  // the block's R tokens at a time share columns: added in order, one slab per block (a lone block: the gradients themselves)
 #pragma unroll
-  for (int q = 0; q < 2; ++q)
+  for (int q = 0; q < 2; ++q) {
+    float* p = norm_slab(a, q);
+    if (!p) continue;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int c0 = E * (l + G * v);
@@ -315,9 +321,10 @@ __global__ __launch_bounds__(NormRowsBlock<G>::T) void norm_rows_bwd_kernel(Norm
 #pragma unroll
         for (int h = 0; h < E; h += 4) {
           const float four[4] = {o[h], o[h + 1], o[h + 2], o[h + 3]};
-          VecIo<float>::store(p + q * C + c0 + h, four, n[v] - h);
+          VecIo<float>::store(p + c0 + h, four, n[v] - h);
         }
     }
+  }
 }
 
 // Planar maps: PX lanes along the pixels (E consecutive pixels of a channel, 16 bytes, per lane), T / PX groups of lanes over the
@@ -517,8 +524,8 @@ __global__ __launch_bounds__(T) void norm_planar_bwd_kernel(NormArgs a) {
       if (cg + CG * k < C) VecIo<AT>::store(reinterpret_cast<AT*>(a.y) + (row0 + CG * k) * P + t0 + yoff, y, n);
     }
   }
-  if (!a.partial) return;
-  float* p = a.partial + (int64_t)blockIdx.x * 2 * C;
+  float* pw = norm_slab(a, 0);
+  float* pb = norm_slab(a, 1);
 #pragma unroll
   for (int k = 0; k < NC; ++k) {
     float u = dw[k], v = db[k];
@@ -527,7 +534,10 @@ __global__ __launch_bounds__(T) void norm_planar_bwd_kernel(NormArgs a) {
     if (PX >= 4) { u += csn_lane_xor_f32<2>(u); v += csn_lane_xor_f32<2>(v); }
     u += csn_lane_xor_f32<1>(u); v += csn_lane_xor_f32<1>(v);
     const int c = cg + CG * k;
-    if (px == 0 && c < C) { p[c] = u; p[C + c] = v; }
+    if (px == 0 && c < C) {
+      if (pw) pw[c] = u;
+      if (pb) pb[c] = v;
+    }
   }
 }
 
@@ -687,7 +697,7 @@ int csn_launch_norm_bwd(const NormArgs& a0, int rows, int a16, int fmt, void* st
   if (p.slabs > 0) {
     if (!a.dweight && !a.dbias) a.partial = nullptr;
     const int e = norm_fast(a, p, rows, a16, a.x ? NORM_X : fmt, true, stream);
-    if (e != 0 || !a.partial) return e;
+    if (e != 0 || !a.partial || p.slabs == 1) return e;
     a.slabs = (int32_t)p.slabs;
     CSN_LAUNCH(norm_reduce_kernel, dim3((unsigned)((2 * a.C + 63) / 64)), dim3(1024), 1024 * sizeof(double), stream, a);
     return (int)hipGetLastError();
@@ -702,5 +712,6 @@ int csn_launch_norm_bwd(const NormArgs& a0, int rows, int a16, int fmt, void* st
 }
 
 int64_t csn_norm_partial_floats(int rows, int a16, int64_t outer, int64_t C, int64_t inner) {
-  return norm_plan(rows, a16, true, outer, C, inner, 0, 0).slabs * 2 * C;   // (strides only ever lower the count)
+  const int64_t slabs = norm_plan(rows, a16, true, outer, C, inner, 0, 0).slabs;   // (strides only ever lower the count)
+  return slabs > 1 ? slabs * 2 * C : 0;
 }

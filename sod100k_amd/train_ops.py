@@ -9,14 +9,13 @@ planar maps ``[B, C, ...]`` (the framework's layout), ``-1`` for rows of tokens 
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
+import math
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 
 from . import _native as N
-from .engine import _stream_of
 
 _DTYPES = {torch.float32: N.DTYPE_F32, torch.bfloat16: N.DTYPE_BF16}
 _FORMATS = {"int8": N.Q8_INT8, "e4m3": N.Q8_E4M3}
@@ -43,25 +42,30 @@ def _dtype(t: torch.Tensor, what: str) -> int:
     return _DTYPES[t.dtype]
 
 
-def _same_device(lib: C.CDLL, *tensors: Optional[torch.Tensor]) -> torch.device:
+def _same_device(lib: C.CDLL, first: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.device:
     """The tensors' one device.  The product library works on ROCm tensors only (no CPU fallback)."""
-    dev = None
-    for t in tensors:
-        if t is None:
-            continue
-        if dev is not None and t.device != dev:
+    dev = first.device
+    for t in others:
+        if t is not None and t.device != dev:
             raise ValueError(f"tensors on different devices: {dev} and {t.device}")
-        dev = t.device
     if (dev.type == "cuda") != (lib is N._lib):
         raise RuntimeError(f"this library does not work on {dev.type} tensors (the HIP path is ROCm only: there is no CPU fallback)")
     return dev
 
 
-def _on(dev: torch.device):
-    """Launches go to the device that is current: make it the tensors' own."""
-    if dev.type == "cuda" and torch.cuda.current_device() != dev.index:
-        return torch.cuda.device(dev)
-    return contextlib.nullcontext()
+def _launch(lib: C.CDLL, dev: torch.device, what: str, *args) -> None:
+    """Call entry point ``what`` with ``args`` and the current stream of ``dev``, which is made current if another device is (a
+    launch goes to the device that is current)."""
+    fn = getattr(lib, what)
+    if dev.type != "cuda":
+        st = fn(*args, None)
+    elif torch.cuda.current_device() == dev.index:
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if st:
+        N.check(lib, st, what)
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -82,6 +86,9 @@ def _channel_axis(dim: int, ndim: int) -> bool:
 def _view(x: torch.Tensor, rows: bool) -> Tuple[torch.Tensor, int, int]:
     """(tensor, outer stride, channel stride) of x as [tokens][C] or [B][C][pixels] with consecutive innermost elements; slices of
     wider tensors are taken as they lie, anything else is copied."""
+    if x.is_contiguous():
+        ch = x.shape[-1] if rows else x.shape[1]
+        return (x, ch, 0) if rows else (x, x.numel() // x.shape[0], x.numel() // (x.shape[0] * ch))
     v = x.reshape(-1, x.shape[-1]) if rows else x.flatten(2)
     if v.shape[-1] > 1 and v.stride(-1) != 1:
         v = v.contiguous()
@@ -94,10 +101,9 @@ def _blocks(cols: int) -> int:
 
 
 def _scales_shape(shape, start_dim: int) -> Tuple[int, ...]:
-    cols = 1
-    for s in shape[start_dim:]:
-        cols *= s
-    return tuple(shape[:start_dim]) + (_blocks(cols),)
+    if start_dim == -1:
+        return tuple(shape[:-1]) + (_blocks(shape[-1]),)
+    return tuple(shape[:start_dim]) + (_blocks(math.prod(shape[start_dim:])),)
 
 
 def _check_q8(q: Q8) -> int:
@@ -114,9 +120,7 @@ def _check_q8(q: Q8) -> int:
 
 
 def _q8_rows(q: Q8) -> Tuple[int, int]:
-    cols = 1
-    for s in q.codes.shape[q.start_dim:]:
-        cols *= s
+    cols = math.prod(q.codes.shape[q.start_dim:])
     return (q.codes.numel() // cols if cols else 0), cols
 
 
@@ -128,14 +132,13 @@ def q8_pack(lib: C.CDLL, x: torch.Tensor, format: str = "int8", start_dim: int =
     if start_dim not in (2, -1) or x.dim() < (3 if start_dim == 2 else 1):
         raise ValueError("start_dim is -1 (the last axis) or 2 (the pixels of planar maps [B, C, ...])")
     rows = start_dim == -1
-    codes = torch.empty(x.shape, dtype=torch.uint8, device=dev)
-    scales = torch.empty(_scales_shape(x.shape, start_dim), dtype=torch.uint8, device=dev)
+    codes = x.new_empty(x.shape, dtype=torch.uint8)
+    scales = x.new_empty(_scales_shape(x.shape, start_dim), dtype=torch.uint8)
     if x.numel():
         v, so, sc = _view(x, rows)
-        o, r, c, s0, s1 = (1, v.shape[0], v.shape[1], 0, so) if rows else (v.shape[0], v.shape[1], v.shape[2], so, sc)
-        with _on(dev):
-            N.check(lib, lib.csn_q8_pack(v.data_ptr(), dt, o, r, c, s0, s1, f, codes.data_ptr(), scales.data_ptr(), _stream_of(x)),
-                    "csn_q8_pack")
+        ch = x.shape[-1] if rows else x.shape[1]
+        o, r, c, s0, s1 = (1, x.numel() // ch, ch, 0, so) if rows else (x.shape[0], ch, x.numel() // (x.shape[0] * ch), so, sc)
+        _launch(lib, dev, "csn_q8_pack", v.data_ptr(), dt, o, r, c, s0, s1, f, codes.data_ptr(), scales.data_ptr())
     return Q8(codes, scales, format, start_dim)
 
 
@@ -143,13 +146,11 @@ def q8_unpack(lib: C.CDLL, q: Q8, dtype: torch.dtype = torch.float32) -> torch.T
     """The values of a checkpoint as a dense float32 or bfloat16 tensor (both hold them exactly)."""
     f = _check_q8(q)
     dev = _same_device(lib, q.codes, q.scales)
-    y = torch.empty(q.codes.shape, dtype=dtype, device=dev)
+    y = q.codes.new_empty(q.codes.shape, dtype=dtype)
     dt = _dtype(y, "q8_unpack")
     if y.numel():
         rows, cols = _q8_rows(q)
-        with _on(dev):
-            N.check(lib, lib.csn_q8_unpack(q.codes.data_ptr(), q.scales.data_ptr(), f, rows, cols, y.data_ptr(), dt, _stream_of(y)),
-                    "csn_q8_unpack")
+        _launch(lib, dev, "csn_q8_unpack", q.codes.data_ptr(), q.scales.data_ptr(), f, rows, cols, y.data_ptr(), dt)
     return y
 
 
@@ -160,17 +161,16 @@ def _param(t: Optional[torch.Tensor], channels: int, what: str) -> Optional[torc
         raise TypeError(f"{what}: float32 expected, got {t.dtype}")
     if tuple(t.shape) != (channels,):
         raise ValueError(f"{what}: shape ({channels},) expected, got {tuple(t.shape)}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _norm_desc(rows: bool, dt: int, shape, eps: float, fmt: int) -> N.NormDesc:
     d = N.NormDesc()
     d.layout, d.dtype, d.eps, d.format = (N.LAYOUT_ROWS if rows else N.LAYOUT_PLANAR), dt, float(eps), fmt
-    d.outer, d.channels, d.inner = 1, (shape[-1] if rows else shape[1]), 1
-    for s in (shape[:-1] if rows else shape[:1]):
-        d.outer *= s
-    for s in (() if rows else shape[2:]):
-        d.inner *= s
+    if rows:
+        d.outer, d.channels, d.inner = math.prod(shape[:-1]), shape[-1], 1
+    else:
+        d.outer, d.channels, d.inner = shape[0], shape[1], math.prod(shape[2:])
     return d
 
 
@@ -187,20 +187,19 @@ def layer_norm_forward(lib: C.CDLL, x: torch.Tensor, weight: Optional[torch.Tens
     dev = _same_device(lib, x, weight, bias)
     fmt = _format(checkpoint) if checkpoint is not None else 0
     d = _norm_desc(rows, dt, x.shape, eps, fmt)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    y = x.new_empty(x.shape)
     sshape = x.shape[:-1] if rows else x.shape[:1] + x.shape[2:]
-    mean = torch.empty(sshape, dtype=torch.float32, device=dev)
-    rstd = torch.empty(sshape, dtype=torch.float32, device=dev)
-    q = None
+    mean = x.new_empty(sshape, dtype=torch.float32)
+    rstd = x.new_empty(sshape, dtype=torch.float32)
+    q = codes = scales = None
     if checkpoint is not None:
         start = -1 if rows else 2
-        q = Q8(torch.empty(x.shape, dtype=torch.uint8, device=dev),
-               torch.empty(_scales_shape(x.shape, start), dtype=torch.uint8, device=dev), checkpoint, start)
+        q = Q8(x.new_empty(x.shape, dtype=torch.uint8), x.new_empty(_scales_shape(x.shape, start), dtype=torch.uint8), checkpoint, start)
+        if x.numel():
+            codes, scales = q.codes.data_ptr(), q.scales.data_ptr()
     v, so, sc = _view(x, rows) if x.numel() else (x, 0, 0)
-    with _on(dev):
-        N.check(lib, lib.csn_layer_norm_forward(C.byref(d), v.data_ptr(), so, sc, _ptr(weight), _ptr(bias), y.data_ptr(),
-                                                mean.data_ptr(), rstd.data_ptr(), _ptr(q.codes) if q and x.numel() else None,
-                                                _ptr(q.scales) if q and x.numel() else None, _stream_of(x)), "csn_layer_norm_forward")
+    _launch(lib, dev, "csn_layer_norm_forward", C.byref(d), v.data_ptr(), so, sc, _ptr(weight), _ptr(bias), y.data_ptr(),
+            mean.data_ptr(), rstd.data_ptr(), codes, scales)
     return y, mean, rstd, q
 
 
@@ -229,19 +228,20 @@ def layer_norm_backward(lib: C.CDLL, dy: torch.Tensor, x: Union[torch.Tensor, Q8
     mean, rstd = mean.contiguous(), rstd.contiguous()
     dev = _same_device(lib, dy, src, q.scales if q is not None else None, mean, rstd, weight)
     d = _norm_desc(rows, dt, dy.shape, 1.0, fmt)
-    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev)
-    dweight = torch.empty(ch, dtype=torch.float32, device=dev)
-    dbias = torch.empty(ch, dtype=torch.float32, device=dev)
-    nbytes = int(lib.csn_layer_norm_workspace_bytes(C.byref(d)))
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    dx = dy.new_empty(dy.shape)
+    dweight = dy.new_empty((ch,), dtype=torch.float32)
+    dbias = dy.new_empty((ch,), dtype=torch.float32)
+    nbytes = lib.csn_layer_norm_workspace_bytes(C.byref(d))
+    ws = dy.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
     vd, dso, dsc = _view(dy, rows) if dy.numel() else (dy, 0, 0)
-    vx, so, sc = _view(x, rows) if q is None and dy.numel() else (None, 0, 0)
-    with _on(dev):
-        N.check(lib, lib.csn_layer_norm_backward(C.byref(d), vd.data_ptr(), dso, dsc, _ptr(vx), so, sc,
-                                                 _ptr(q.codes) if q is not None and dy.numel() else None,
-                                                 _ptr(q.scales) if q is not None and dy.numel() else None, mean.data_ptr(),
-                                                 rstd.data_ptr(), _ptr(weight), dx.data_ptr(), dweight.data_ptr(),
-                                                 dbias.data_ptr(), _ptr(ws), nbytes, _stream_of(dy)), "csn_layer_norm_backward")
+    vx, so, sc, codes, scales = None, 0, 0, None, None
+    if dy.numel():
+        if q is None:
+            vx, so, sc = _view(x, rows)
+        else:
+            codes, scales = q.codes.data_ptr(), q.scales.data_ptr()
+    _launch(lib, dev, "csn_layer_norm_backward", C.byref(d), vd.data_ptr(), dso, dsc, _ptr(vx), so, sc, codes, scales, mean.data_ptr(),
+            rstd.data_ptr(), _ptr(weight), dx.data_ptr(), dweight.data_ptr(), dbias.data_ptr(), _ptr(ws), nbytes)
     return dx, dweight, dbias
 
 
@@ -261,15 +261,13 @@ def product_weight_grad(lib: C.CDLL, dy: torch.Tensor, q: Q8, dim: int = -1) -> 
     d = N.ProductDesc()
     d.layout, d.dtype, d.format, d.outer, d.inner = nd.layout, dt, fmt, nd.outer, nd.inner
     d.cin, d.cout = (xs[-1], ds[-1]) if rows else (xs[1], ds[1])
-    dweight = torch.empty((d.cout, d.cin), dtype=torch.float32, device=dev)
-    dbias = torch.empty(d.cout, dtype=torch.float32, device=dev)
-    nbytes = int(lib.csn_product_weight_grad_workspace_bytes(C.byref(d)))
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    dweight = dy.new_empty((d.cout, d.cin), dtype=torch.float32)
+    dbias = dy.new_empty((d.cout,), dtype=torch.float32)
+    nbytes = lib.csn_product_weight_grad_workspace_bytes(C.byref(d))
+    ws = dy.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
     v, so, sc = _view(dy, rows) if dy.numel() else (dy, 0, 0)
-    with _on(dev):
-        N.check(lib, lib.csn_product_weight_grad(C.byref(d), v.data_ptr(), so, sc, q.codes.data_ptr(), q.scales.data_ptr(),
-                                                 dweight.data_ptr(), dbias.data_ptr(), _ptr(ws), nbytes, _stream_of(dy)),
-                "csn_product_weight_grad")
+    _launch(lib, dev, "csn_product_weight_grad", C.byref(d), v.data_ptr(), so, sc, q.codes.data_ptr(), q.scales.data_ptr(),
+            dweight.data_ptr(), dbias.data_ptr(), _ptr(ws), nbytes)
     return dweight, dbias
 
 
