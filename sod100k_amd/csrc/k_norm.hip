@@ -6,6 +6,7 @@
 // with xh = (x - mean) rstd; in the backward x may be the 8-bit checkpoint that the forward left (q8_core.h).
 #include "csn_reduce.h"
 #include "q8_core.h"
+#include "slab_sum.h"
 #include "train_ops.h"
 #include "vec_io.h"
 
@@ -134,39 +135,59 @@ __device__ __forceinline__ float* norm_slab(const NormArgs& a, int q) {
   return a.partial ? a.partial + ((int64_t)blockIdx.x * 2 + q) * a.C : nullptr;
 }
 
+// E weights (or biases) of a piece, `none` past the row's end or without a tensor
+template <int E>
+__device__ __forceinline__ void norm_param(float (&f)[E], const float* p, int n, float none) {
+#pragma unroll
+  for (int h = 0; h < E; h += 4) {
+    VecIo<float> v;
+    v.zero();
+    if (p && n - h >= 4) v.load(p + h);
+    else if (p) v.load_each(p + h, n - h);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[h + j] = p && h + j < n ? csn_bits_f(v.w[j]) : none;
+  }
+}
+
 template <int G> struct NormRowsBlock { static constexpr int T = G > CSN_BLOCK ? G : CSN_BLOCK; };
 
 // Rows of tokens: G lanes per token, NV pieces of E elements (16 bytes) per lane.  A block walks tokens, its weights in registers.
-template <typename AT, int G, int NV, int CK>
+// W: a token has at least E channels
+template <typename AT, int G, int NV, bool W, int CK>
 __global__ __launch_bounds__(NormRowsBlock<G>::T) void norm_rows_fwd_kernel(NormArgs a) {
   constexpr int E = VecIo<AT>::E, T = NormRowsBlock<G>::T, R = T / G;
   CSN_DYN_SMEM(float, sm);
   const int l = threadIdx.x % G, C = (int)a.C;
   const float inv_c = 1.f / (float)C;
-  const bool wide = C >= E;
   float w[NV][E], b[NV][E];
   int n[NV];
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     const int c0 = E * (l + G * v);
     n[v] = C - c0;
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-      w[v][j] = a.weight && j < n[v] ? a.weight[c0 + j] : 1.f;
-      b[v][j] = a.bias && j < n[v] ? a.bias[c0 + j] : 0.f;
-    }
+    norm_param<E>(w[v], a.weight ? a.weight + c0 : nullptr, n[v], 1.f);
+    norm_param<E>(b[v], a.bias ? a.bias + c0 : nullptr, n[v], 0.f);
   }
   int turn = 0;
-  for (int64_t t = (int64_t)blockIdx.x * R + threadIdx.x / G; t < a.outer; t += (int64_t)gridDim.x * R) {
-    const AT* x = reinterpret_cast<const AT*>(a.x) + t * a.x_so;
+  const int64_t step = (int64_t)gridDim.x * R;
+  int64_t t = (int64_t)blockIdx.x * R + threadIdx.x / G;
+  VecIo<AT> nx[NV];
+  auto load = [&](int64_t row) {
+    const AT* x = reinterpret_cast<const AT*>(a.x) + row * a.x_so;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) vec_load<W>(nx[v], x + E * (l + G * v), n[v]);
+  };
+  if (t < a.outer) load(t);
+  for (; t < a.outer; t += step) {
     VecIo<AT> r[NV];
 #pragma unroll
-    for (int v = 0; v < NV; ++v) vec_load(r[v], x + E * (l + G * v), n[v], wide);
+    for (int v = 0; v < NV; ++v) r[v] = nx[v];
+    if (t + step < a.outer) load(t + step);   // (in flight while this token is worked on)
     float s[1] = {0.f};
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       float f[E];
-      vec_end(r[v], n[v], wide);
+      vec_end<W>(r[v], n[v]);
       r[v].get(f);
 #pragma unroll
       for (int j = 0; j < E; ++j) s[0] += f[j];
@@ -211,64 +232,71 @@ __global__ __launch_bounds__(NormRowsBlock<G>::T) void norm_rows_fwd_kernel(Norm
 }
 
 // one piece of the backward's input, the tensor or its checkpoint
-template <typename AT, int SRC> struct NormIn {
-  static constexpr int E = VecIo<AT>::E;
+template <typename AT, int E, int SRC> struct NormIn {
   CodeIo<E> c;
-  float scale;
-  __device__ __forceinline__ void end(int n, bool wide) { code_end<E>(c, n, wide); }
+  unsigned e;
+  template <bool W> __device__ __forceinline__ void end(int n) { code_end<W, E>(c, n); }
   __device__ __forceinline__ void pin() { c.pin(); }
-  __device__ __forceinline__ void get(float (&f)[E]) const { q8_decode_vec<SRC, E>(c.w, scale, f); }
+  __device__ __forceinline__ void get(float (&f)[E]) const { q8_decode_vec<SRC, E>(c.w, q8_scale(e), f); }
 };
-template <typename AT> struct NormIn<AT, NORM_X> {
-  static constexpr int E = VecIo<AT>::E;
-  VecIo<AT> v;
-  __device__ __forceinline__ void end(int n, bool wide) { vec_end(v, n, wide); }
+template <typename AT, int E> struct NormIn<AT, E, NORM_X> {
+  VecIo<AT, E> v;
+  template <bool W> __device__ __forceinline__ void end(int n) { vec_end<W>(v, n); }
   __device__ __forceinline__ void pin() { v.pin(); }
   __device__ __forceinline__ void get(float (&f)[E]) const { v.get(f); }
 };
 
-template <typename AT, int G, int NV, int SRC>
+template <typename AT, int G, int NV, bool W, int SRC>
 __global__ __launch_bounds__(NormRowsBlock<G>::T) void norm_rows_bwd_kernel(NormArgs a) {
   constexpr int E = VecIo<AT>::E, T = NormRowsBlock<G>::T, R = T / G;
   CSN_DYN_SMEM(float, sm);
   const int l = threadIdx.x % G, C = (int)a.C;
   const float inv_c = 1.f / (float)C;
-  const bool wide = C >= E;
   float w[NV][E], dw[NV][E], db[NV][E];
   int n[NV];
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     const int c0 = E * (l + G * v);
     n[v] = C - c0;
+    norm_param<E>(w[v], a.weight ? a.weight + c0 : nullptr, n[v], 1.f);
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      w[v][j] = a.weight && j < n[v] ? a.weight[c0 + j] : 1.f;
-      dw[v][j] = db[v][j] = 0.f;
-    }
+    for (int j = 0; j < E; ++j) dw[v][j] = db[v][j] = 0.f;
   }
   int turn = 0;
-  for (int64_t t = (int64_t)blockIdx.x * R + threadIdx.x / G; t < a.outer; t += (int64_t)gridDim.x * R) {
-    const AT* dy = reinterpret_cast<const AT*>(a.dy) + t * a.dy_so;
-    NormIn<AT, SRC> rx[NV];
-    VecIo<AT> rd[NV];
+  const int64_t step = (int64_t)gridDim.x * R;
+  int64_t t = (int64_t)blockIdx.x * R + threadIdx.x / G;
+  NormIn<AT, E, SRC> nx[NV];
+  VecIo<AT> nd[NV];
+  float nmean = 0.f, nrstd = 0.f;
+  auto load = [&](int64_t row) {
+    const AT* dy = reinterpret_cast<const AT*>(a.dy) + row * a.dy_so;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int c0 = E * (l + G * v);
       if constexpr (SRC == NORM_X) {
-        vec_load(rx[v].v, reinterpret_cast<const AT*>(a.x) + t * a.x_so + c0, n[v], wide);
+        vec_load<W>(nx[v].v, reinterpret_cast<const AT*>(a.x) + row * a.x_so + c0, n[v]);
       } else {
-        code_load<E>(rx[v].c, a.codes_in + t * C + c0, n[v], wide);
-        rx[v].scale = n[v] > 0 ? q8_scale(a.exps_in[t * a.nblk + (c0 >> 5)]) : 1.f;
+        code_load<W, E>(nx[v].c, a.codes_in + row * C + c0, n[v]);
+        nx[v].e = n[v] > 0 ? a.exps_in[row * a.nblk + (c0 >> 5)] : 127;
       }
-      vec_load(rd[v], dy + c0, n[v], wide);
+      vec_load<W>(nd[v], dy + c0, n[v]);
     }
-    const float mean = a.mean[t], rstd = a.rstd[t];
+    nmean = a.mean[row]; nrstd = a.rstd[row];
+  };
+  if (t < a.outer) load(t);
+  for (; t < a.outer; t += step) {
+    NormIn<AT, E, SRC> rx[NV];
+    VecIo<AT> rd[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) { rx[v] = nx[v]; rd[v] = nd[v]; }
+    const float mean = nmean, rstd = nrstd;
+    if (t + step < a.outer) load(t + step);   // (in flight while this token is worked on)
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       float f[E], d[E];
-      rx[v].end(n[v], wide);
-      vec_end(rd[v], n[v], wide);
+      rx[v].template end<W>(n[v]);
+      vec_end<W>(rd[v], n[v]);
       rx[v].get(f);
       rd[v].get(d);
 #pragma unroll
@@ -327,9 +355,10 @@ __global__ __launch_bounds__(NormRowsBlock<G>::T) void norm_rows_bwd_kernel(Norm
   }
 }
 
-// Planar maps: PX lanes along the pixels (E consecutive pixels of a channel, 16 bytes, per lane), T / PX groups of lanes over the
-// channels, NC channels per lane in registers.  Sums over a pixel's channels: butterfly over the groups of a wave, then the waves in
+// Planar maps: PX lanes along the pixels (four consecutive pixels of a channel per lane: eight would double the statistics that
+// every lane carries), T / PX groups of lanes over the channels, NC channels per lane in registers.  Sums over a pixel's channels: butterfly over the groups of a wave, then the waves in
 // order through LDS (two buffers of [waves][N][PX * E] floats in turn).
+#define NORM_PE 4
 template <int T, int PX, int E, int N>
 __device__ __forceinline__ void norm_planar_sum(float (&v)[N][E], float* sm, int& turn) {
   constexpr int W = T / 64, TP = PX * E;
@@ -356,7 +385,7 @@ __device__ __forceinline__ void norm_planar_sum(float (&v)[N][E], float* sm, int
   for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int j = 0; j < E; ++j) v[i][j] = 0.f;
-#pragma unroll 2   // (all at once would hold T / 4 registers)
+#pragma unroll 2
   for (int k = 0; k < W; ++k)
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -364,15 +393,24 @@ __device__ __forceinline__ void norm_planar_sum(float (&v)[N][E], float* sm, int
       for (int j = 0; j < E; ++j) v[i][j] += b[(k * N + i) * TP + px * E + j];
 }
 
-// (image, pixel tile) items of a persistent launch.  Addresses are a uniform base -- image, tile, group of channels k -- plus one
-// 32-bit offset per lane that all of its channels share.
+// (image, pixel tile) items of a persistent launch.  Addresses are a uniform base -- image, group of channels k -- plus one 32-bit
+// byte offset per lane that all of its channels share (64-bit addresses per channel would cost two registers each).
+template <typename T>
+__device__ __forceinline__ T* norm_at(T* base, unsigned bytes) {
+  return reinterpret_cast<T*>(reinterpret_cast<typename std::conditional<std::is_const<T>::value, const char, char>::type*>(base) + bytes);
+}
+// n pixels (n <= 0: none) of a lane whose byte offset is that of its piece stepped back as far as vec_load would
+template <typename AT, int E>
+__device__ __forceinline__ void norm_load(VecIo<AT, E>& v, const AT* base, unsigned bytes, int n) {
+  v.zero();
+  if (n > 0) v.load(norm_at(base, bytes));
+}
 template <typename AT, int T, int PX, int NC, int CK>
 __global__ __launch_bounds__(T) void norm_planar_fwd_kernel(NormArgs a) {
-  constexpr int E = VecIo<AT>::E, CG = T / PX, TP = PX * E;
+  constexpr int E = NORM_PE, CG = T / PX, TP = PX * E;
   CSN_DYN_SMEM(float, sm);
   const int px = threadIdx.x % PX, cg = threadIdx.x / PX, C = (int)a.C, P = (int)a.inner;
   const float inv_c = 1.f / (float)C;
-  const bool wide = P >= E;
   float w[NC], b[NC];
 #pragma unroll
   for (int k = 0; k < NC; ++k) {
@@ -380,25 +418,31 @@ __global__ __launch_bounds__(T) void norm_planar_fwd_kernel(NormArgs a) {
     w[k] = a.weight && c < C ? a.weight[c] : 1.f;
     b[k] = a.bias && c < C ? a.bias[c] : 0.f;
   }
-  const unsigned xoff = (unsigned)cg * (unsigned)a.x_sc + px * E, yoff = (unsigned)cg * (unsigned)P + px * E;
+  constexpr unsigned ES = sizeof(AT);
+  const unsigned xlane = (unsigned)cg * (unsigned)a.x_sc + px * E, ylane = (unsigned)cg * (unsigned)P + px * E;
   int turn = 0;
   for (int it = blockIdx.x; it < a.items; it += gridDim.x) {
     const int o = it / a.tiles, t0 = (it - o * a.tiles) * TP;
     const int n = P - t0 - px * E;
-    const AT* x = reinterpret_cast<const AT*>(a.x) + o * a.x_so + t0;
-    VecIo<AT> r[NC];
+    const AT* x = reinterpret_cast<const AT*>(a.x) + o * a.x_so;
+    const unsigned xoff = (xlane + t0 - vec_back(n > 0 ? n : E, E)) * ES, yoff = ylane + t0;
+    VecIo<AT, E> r[NC];
 #pragma unroll
-    for (int k = 0; k < NC; ++k) vec_load(r[k], x + (int64_t)(CG * k) * a.x_sc + xoff, cg + CG * k < C ? n : 0, wide);
+    for (int k = 0; k < NC; ++k) norm_load(r[k], x + (int64_t)(CG * k) * a.x_sc, xoff, cg + CG * k < C ? n : 0);
+    if (t0 + TP > P)   // (the image's last tile, one branch for all channels: the sums below stay one straight block)
+#pragma unroll
+      for (int k = 0; k < NC; ++k) vec_end<true>(r[k], n);
     float s[1][E];
 #pragma unroll
     for (int j = 0; j < E; ++j) s[0][j] = 0.f;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       float f[E];
-      vec_end(r[k], n, wide);
+      r[k].pin();
       r[k].get(f);
 #pragma unroll
       for (int j = 0; j < E; ++j) s[0][j] += f[j];
+      CSN_SCHED_FENCE();   // one channel's floats at a time in registers
     }
     norm_planar_sum<T, PX, E, 1>(s, sm, turn);
     float mean[E], rstd[E];
@@ -409,9 +453,12 @@ __global__ __launch_bounds__(T) void norm_planar_fwd_kernel(NormArgs a) {
       float f[E];
       r[k].pin();
       r[k].get(f);
-      if (cg + CG * k < C)
 #pragma unroll
-        for (int j = 0; j < E; ++j) s[0][j] = fmaf(f[j] - mean[j], f[j] - mean[j], s[0][j]);
+      for (int j = 0; j < E; ++j) {
+        const float d = cg + CG * k < C ? f[j] - mean[j] : 0.f;
+        s[0][j] = fmaf(d, d, s[0][j]);
+      }
+      CSN_SCHED_FENCE();
     }
     norm_planar_sum<T, PX, E, 1>(s, sm, turn);
 #pragma unroll
@@ -425,16 +472,18 @@ __global__ __launch_bounds__(T) void norm_planar_fwd_kernel(NormArgs a) {
       r[k].get(f);
 #pragma unroll
       for (int j = 0; j < E; ++j) y[j] = fmaf((f[j] - mean[j]) * rstd[j], w[k], b[k]);
-      const int64_t base = (row0 + CG * k) * P + t0;
-      if (c < C) VecIo<AT>::store(reinterpret_cast<AT*>(a.y) + base + yoff, y, n);
+      const int64_t base = (row0 + CG * k) * P;
+      if (c < C) VecIo<AT, E>::store(norm_at(reinterpret_cast<AT*>(a.y) + base, yoff * ES), y, n);
       if (CK >= 0) {
         unsigned q[E / 4];
         const unsigned e = q8_pack_block<CK, E>(f, q);
         if (c < C) {
-          code_store<E>(a.codes + base + yoff, q, n);
-          if ((px & (32 / E - 1)) == 0 && n > 0) a.exps[(row0 + c) * a.nblk + ((t0 + px * E) >> 5)] = (uint8_t)e;
+          code_store<E>(norm_at(a.codes + base, yoff), q, n);
+          if ((px & (32 / E - 1)) == 0 && n > 0)
+            *norm_at(a.exps + (row0 + CG * k) * a.nblk, (unsigned)cg * (unsigned)a.nblk + ((t0 + px * E) >> 5)) = (uint8_t)e;
         }
       }
+      CSN_SCHED_FENCE();
     }
     if (cg == 0) {
       const int64_t st = (int64_t)o * P + t0 + px * E;
@@ -452,38 +501,45 @@ __global__ __launch_bounds__(T) void norm_planar_fwd_kernel(NormArgs a) {
 
 template <typename AT, int T, int PX, int NC, int SRC>
 __global__ __launch_bounds__(T) void norm_planar_bwd_kernel(NormArgs a) {
-  constexpr int E = VecIo<AT>::E, CG = T / PX, TP = PX * E;
+  constexpr int E = NORM_PE, CG = T / PX, TP = PX * E;
   CSN_DYN_SMEM(float, sm);
   const int px = threadIdx.x % PX, cg = threadIdx.x / PX, C = (int)a.C, P = (int)a.inner;
   const float inv_c = 1.f / (float)C;
-  const bool wide = P >= E;
   float w[NC], dw[NC], db[NC];
 #pragma unroll
   for (int k = 0; k < NC; ++k) {
     w[k] = a.weight && cg + CG * k < C ? a.weight[cg + CG * k] : 1.f;
     dw[k] = db[k] = 0.f;
   }
-  const unsigned xoff = (unsigned)cg * (unsigned)a.x_sc + px * E, doff = (unsigned)cg * (unsigned)a.dy_sc + px * E;
-  const unsigned yoff = (unsigned)cg * (unsigned)P + px * E;
+  constexpr unsigned ES = sizeof(AT);
+  const unsigned xlane = (unsigned)cg * (unsigned)a.x_sc + px * E, dlane = (unsigned)cg * (unsigned)a.dy_sc + px * E;
+  const unsigned ylane = (unsigned)cg * (unsigned)P + px * E;
   int turn = 0;
   for (int it = blockIdx.x; it < a.items; it += gridDim.x) {
     const int o = it / a.tiles, t0 = (it - o * a.tiles) * TP;
     const int n = P - t0 - px * E;
     const int64_t row0 = (int64_t)o * C;
-    const AT* x = reinterpret_cast<const AT*>(a.x) + o * a.x_so + t0;
-    const AT* dy = reinterpret_cast<const AT*>(a.dy) + o * a.dy_so + t0;
-    NormIn<AT, SRC> rx[NC];
-    VecIo<AT> rd[NC];
+    const AT* x = reinterpret_cast<const AT*>(a.x) + o * a.x_so;
+    const AT* dy = reinterpret_cast<const AT*>(a.dy) + o * a.dy_so;
+    const int tb = t0 - vec_back(n > 0 ? n : E, E);
+    const unsigned xoff = (xlane + tb) * ES, doff = (dlane + tb) * ES, coff = ylane + tb, yoff = (ylane + t0) * ES;
+    const unsigned eoff = (unsigned)cg * (unsigned)a.nblk + ((t0 + px * E) >> 5);
+    NormIn<AT, E, SRC> rx[NC];
+    VecIo<AT, E> rd[NC];
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       const int m = cg + CG * k < C ? n : 0;
       if constexpr (SRC == NORM_X) {
-        vec_load(rx[k].v, x + (int64_t)(CG * k) * a.x_sc + xoff, m, wide);
+        norm_load(rx[k].v, x + (int64_t)(CG * k) * a.x_sc, xoff, m);
       } else {
-        code_load<E>(rx[k].c, a.codes_in + (row0 + CG * k) * P + t0 + yoff, m, wide);
-        rx[k].scale = m > 0 ? q8_scale(a.exps_in[(row0 + cg + CG * k) * a.nblk + ((t0 + px * E) >> 5)]) : 1.f;
+        rx[k].c.zero();
+        rx[k].e = 127;
+        if (m > 0) {
+          rx[k].c.load(norm_at(a.codes_in + (row0 + CG * k) * P, coff));
+          rx[k].e = *norm_at(a.exps_in + (row0 + CG * k) * a.nblk, eoff);
+        }
       }
-      vec_load(rd[k], dy + (int64_t)(CG * k) * a.dy_sc + doff, m, wide);
+      norm_load(rd[k], dy + (int64_t)(CG * k) * a.dy_sc, doff, m);
     }
     float mean[E], rstd[E], s[2][E];
     const int64_t st = (int64_t)o * P + t0 + px * E;
@@ -493,11 +549,17 @@ __global__ __launch_bounds__(T) void norm_planar_bwd_kernel(NormArgs a) {
       rstd[j] = j < n ? a.rstd[st + j] : 0.f;
       s[0][j] = s[1][j] = 0.f;
     }
+    if (t0 + TP > P)
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        rx[k].template end<true>(n);
+        vec_end<true>(rd[k], n);
+      }
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       float f[E], d[E];
-      rx[k].end(n, wide);
-      vec_end(rd[k], n, wide);
+      rx[k].pin();
+      rd[k].pin();
       rx[k].get(f);
       rd[k].get(d);
 #pragma unroll
@@ -508,6 +570,7 @@ __global__ __launch_bounds__(T) void norm_planar_bwd_kernel(NormArgs a) {
         dw[k] = fmaf(d[j], xh, dw[k]);
         db[k] += d[j];
       }
+      CSN_SCHED_FENCE();   // one channel's floats at a time in registers
     }
     norm_planar_sum<T, PX, E, 2>(s, sm, turn);
 #pragma unroll
@@ -521,7 +584,8 @@ __global__ __launch_bounds__(T) void norm_planar_bwd_kernel(NormArgs a) {
       rd[k].get(d);
 #pragma unroll
       for (int j = 0; j < E; ++j) y[j] = rstd[j] * (fmaf(d[j], w[k], -s[0][j]) - (f[j] - mean[j]) * s[1][j]);
-      if (cg + CG * k < C) VecIo<AT>::store(reinterpret_cast<AT*>(a.y) + (row0 + CG * k) * P + t0 + yoff, y, n);
+      if (cg + CG * k < C) VecIo<AT, E>::store(norm_at(reinterpret_cast<AT*>(a.y) + (row0 + CG * k) * P, yoff), y, n);
+      CSN_SCHED_FENCE();
     }
   }
   float* pw = norm_slab(a, 0);
@@ -541,27 +605,13 @@ __global__ __launch_bounds__(T) void norm_planar_bwd_kernel(NormArgs a) {
   }
 }
 
-// dweight / dbias: the blocks' slabs in order, 64 columns per block, wave w adds slabs w, w + 16, ...
-__global__ __launch_bounds__(1024) void norm_reduce_kernel(NormArgs a) {
-  CSN_DYN_SMEM(double, sd);   // [16][64]
-  const int64_t n = 2 * a.C, e = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-  const int w = threadIdx.x >> 6;
-  double v = 0.0;
-  if (e < n) {
-#pragma unroll 4
-    for (int s = w; s < a.slabs; s += 16) v += a.partial[(int64_t)s * n + e];
-  }
-  sd[w * 64 + (threadIdx.x & 63)] = v;
-  __syncthreads();
-  if (w == 0 && e < n) {
-    for (int q = 1; q < 16; ++q) v += sd[q * 64 + (threadIdx.x & 63)];
-    float* out = e < a.C ? a.dweight : a.dbias;
-    if (out) out[e < a.C ? e : e - a.C] = (float)v;
-  }
-}
-
 // blocks of a persistent launch: the chip's 256 CUs full of waves
+#ifdef NORM_TUNE
+#include <cstdlib>
+static int64_t norm_blocks(int threads) { const char* e = std::getenv("NORM_W"); return 256 * (int64_t)((e ? std::atoi(e) : 2048) / threads); }
+#else
 static int64_t norm_blocks(int threads) { return 256 * (int64_t)(2048 / threads); }
+#endif
 
 // The register forms: which one takes a case, what its grid is.  slabs = 0: none.
 struct NormPlan { int G, NV; int T, PX, NC; int64_t slabs, tiles, items; };
@@ -577,34 +627,35 @@ static NormPlan norm_plan(int rows, int a16, bool bwd, int64_t outer, int64_t C,
     p.slabs = std::min(norm_blocks(p.T), (outer + r - 1) / r);
     return p;
   }
-  if (C > 4096) return p;
-  // the forward holds 16 bytes per channel and lane, the backward 32 and two sums
+  if (C > 2048 || inner < NORM_PE) return p;
+  // 16 lanes of 8 bytes (bfloat16) or 8 of 16 (float) read 128 bytes of a channel; wider tokens than their threads can hold narrow
+  // the tile.  The forward holds one piece per channel and lane, the backward two and two sums
   p.T = C <= 128 ? 256 : C <= 256 ? 512 : 1024;
-  p.PX = C <= 64 ? 16 : C <= 512 ? 8 : bwd ? (C <= 1024 ? 4 : 2) : (C <= 2048 ? 8 : 4);
+  p.PX = a16 ? (C <= 512 ? 16 : C <= 1024 || !bwd ? 8 : 4) : (C <= 512 ? 8 : !bwd ? 8 : C <= 1024 ? 4 : 2);
   const int cg = p.T / p.PX;
   p.NC = C <= 4 * cg ? 4 : C <= 8 * cg ? 8 : 16;
-  const int64_t tile = (int64_t)p.PX * (a16 ? 8 : 4), lim = (int64_t)1 << 30;
+  const int64_t tile = (int64_t)p.PX * NORM_PE, lim = (int64_t)1 << 29;
   p.tiles = (inner + tile - 1) / tile;
   p.items = outer * p.tiles;
-  // 32-bit offsets of a lane and 32-bit item counts
-  if (inner > lim || p.items > lim || cg * std::max(inner, std::max(x_sc, dy_sc)) + tile > lim) { p.slabs = 0; return p; }
+  // 32-bit byte offsets of a lane and 32-bit item counts
+  if (inner > lim || p.items > lim || cg * std::max(inner, std::max(x_sc, dy_sc)) + inner + tile > lim) { p.slabs = 0; return p; }
   p.slabs = std::min(norm_blocks(p.T), p.items);
   return p;
 }
 
-template <typename AT, int G, int NVB, int CK>
+template <typename AT, int G, int NVB, int CK, bool W = true>
 static int norm_rows_go(const NormArgs& a, bool bwd, void* stream) {
   constexpr int NV = NVB * (8 / VecIo<AT>::E), T = NormRowsBlock<G>::T;
   const dim3 g((unsigned)a.slabs), b(T);
   const size_t sm = std::max((size_t)64 * sizeof(float), T / G > 1 ? (size_t)T * VecIo<AT>::E * sizeof(float) : (size_t)0);
-  if (bwd) CSN_LAUNCH((norm_rows_bwd_kernel<AT, G, NV, CK>), g, b, sm, stream, a);
-  else CSN_LAUNCH((norm_rows_fwd_kernel<AT, G, NV, CK>), g, b, sm, stream, a);
+  if (bwd) CSN_LAUNCH((norm_rows_bwd_kernel<AT, G, NV, W, CK>), g, b, sm, stream, a);
+  else CSN_LAUNCH((norm_rows_fwd_kernel<AT, G, NV, W, CK>), g, b, sm, stream, a);
   return (int)hipGetLastError();
 }
 template <typename AT, int CK>
 static int norm_rows_run(const NormArgs& a, const NormPlan& p, bool bwd, void* stream) {
   switch (p.G) {
-    case 8: return norm_rows_go<AT, 8, 1, CK>(a, bwd, stream);
+    case 8: return a.C >= VecIo<AT>::E ? norm_rows_go<AT, 8, 1, CK>(a, bwd, stream) : norm_rows_go<AT, 8, 1, CK, false>(a, bwd, stream);
     case 16: return norm_rows_go<AT, 16, 1, CK>(a, bwd, stream);
     case 32: return norm_rows_go<AT, 32, 1, CK>(a, bwd, stream);
     case 64: return p.NV == 1 ? norm_rows_go<AT, 64, 1, CK>(a, bwd, stream) : norm_rows_go<AT, 64, 2, CK>(a, bwd, stream);
@@ -613,30 +664,36 @@ static int norm_rows_run(const NormArgs& a, const NormPlan& p, bool bwd, void* s
   return p.NV == 1 ? norm_rows_go<AT, 1024, 1, CK>(a, bwd, stream) : norm_rows_go<AT, 1024, 2, CK>(a, bwd, stream);
 }
 template <typename AT, int T, int PX, int NC, int CK>
-static int norm_planar_fwd_go(const NormArgs& a, void* stream) {
-  const size_t sm = (size_t)2 * (T / 64) * PX * VecIo<AT>::E * sizeof(float);
+static int norm_planar_fwd(const NormArgs& a, void* stream) {
+  const size_t sm = (size_t)2 * (T / 64) * PX * NORM_PE * sizeof(float);
   CSN_LAUNCH((norm_planar_fwd_kernel<AT, T, PX, NC, CK>), dim3((unsigned)a.slabs), dim3(T), sm, stream, a);
   return (int)hipGetLastError();
 }
 template <typename AT, int T, int PX, int NC, int CK>
-static int norm_planar_bwd_go(const NormArgs& a, void* stream) {
-  const size_t sm = (size_t)2 * (T / 64) * 2 * PX * VecIo<AT>::E * sizeof(float);
+static int norm_planar_bwd(const NormArgs& a, void* stream) {
+  const size_t sm = (size_t)2 * (T / 64) * 2 * PX * NORM_PE * sizeof(float);
   CSN_LAUNCH((norm_planar_bwd_kernel<AT, T, PX, NC, CK>), dim3((unsigned)a.slabs), dim3(T), sm, stream, a);
   return (int)hipGetLastError();
 }
+template <typename AT, int T, int PX, int NC, int CK>
+static int norm_planar_go(const NormArgs& a, bool bwd, void* stream) {
+  return bwd ? norm_planar_bwd<AT, T, PX, NC, CK>(a, stream) : norm_planar_fwd<AT, T, PX, NC, CK>(a, stream);
+}
 template <typename AT, int CK>
 static int norm_planar_run(const NormArgs& a, const NormPlan& p, bool bwd, void* stream) {
-  if (p.T == 256 && p.PX == 16) return bwd ? norm_planar_bwd_go<AT, 256, 16, 4, CK>(a, stream) : norm_planar_fwd_go<AT, 256, 16, 4, CK>(a, stream);
-  if (p.T == 256) return bwd ? norm_planar_bwd_go<AT, 256, 8, 4, CK>(a, stream) : norm_planar_fwd_go<AT, 256, 8, 4, CK>(a, stream);
-  if (p.T == 512) return bwd ? norm_planar_bwd_go<AT, 512, 8, 4, CK>(a, stream) : norm_planar_fwd_go<AT, 512, 8, 4, CK>(a, stream);
-  if (!bwd) {
-    if (p.NC == 4) return norm_planar_fwd_go<AT, 1024, 8, 4, CK>(a, stream);
-    if (p.NC == 8) return norm_planar_fwd_go<AT, 1024, 8, 8, CK>(a, stream);
-    return p.PX == 8 ? norm_planar_fwd_go<AT, 1024, 8, 16, CK>(a, stream) : norm_planar_fwd_go<AT, 1024, 4, 16, CK>(a, stream);
+  if constexpr (sizeof(AT) == 2) {
+    if (p.T == 256) return p.NC == 4 ? norm_planar_go<AT, 256, 16, 4, CK>(a, bwd, stream) : norm_planar_go<AT, 256, 16, 8, CK>(a, bwd, stream);
+    if (p.T == 512) return norm_planar_go<AT, 512, 16, 8, CK>(a, bwd, stream);
+    if (p.PX == 16) return norm_planar_go<AT, 1024, 16, 8, CK>(a, bwd, stream);
+    if (p.PX == 8 && p.NC == 8) return norm_planar_go<AT, 1024, 8, 8, CK>(a, bwd, stream);
+    return bwd ? norm_planar_bwd<AT, 1024, 4, 8, CK>(a, stream) : norm_planar_fwd<AT, 1024, 8, 16, CK>(a, stream);
+  } else {
+    if (p.T == 256) return norm_planar_go<AT, 256, 8, 4, CK>(a, bwd, stream);
+    if (p.T == 512) return norm_planar_go<AT, 512, 8, 4, CK>(a, bwd, stream);
+    if (p.PX == 8 && p.NC == 4) return norm_planar_go<AT, 1024, 8, 4, CK>(a, bwd, stream);
+    if (p.PX == 8) return p.NC == 8 ? norm_planar_fwd<AT, 1024, 8, 8, CK>(a, stream) : norm_planar_fwd<AT, 1024, 8, 16, CK>(a, stream);
+    return p.PX == 4 ? norm_planar_bwd<AT, 1024, 4, 4, CK>(a, stream) : norm_planar_bwd<AT, 1024, 2, 4, CK>(a, stream);
   }
-  if (p.PX == 8) return norm_planar_bwd_go<AT, 1024, 8, 4, CK>(a, stream);
-  if (p.PX == 4) return norm_planar_bwd_go<AT, 1024, 4, 4, CK>(a, stream);
-  return p.NC == 4 ? norm_planar_bwd_go<AT, 1024, 2, 4, CK>(a, stream) : norm_planar_bwd_go<AT, 1024, 2, 8, CK>(a, stream);
 }
 template <int CK>
 static int norm_fast(const NormArgs& a, const NormPlan& p, int rows, int a16, bool bwd, void* stream) {
@@ -660,12 +717,17 @@ static int norm_fwd(const NormArgs& a, void* stream) {
   return (int)hipGetLastError();
 }
 
+// (maps of one pixel with consecutive channels are rows, but for the blocks of a checkpoint)
+static bool norm_one_pixel(const NormArgs& a, bool bwd) {
+  return a.inner == 1 && !a.codes_in && (a.x_sc == 1 || a.C == 1) && (!bwd || a.dy_sc == 1 || a.C == 1);
+}
+
 int csn_launch_norm_fwd(const NormArgs& a0, int rows, int a16, int fmt, void* stream) {
   NormArgs a = a0;
   if (a.outer * a.inner <= 0) return 0;
-  const NormPlan p = norm_plan(rows, a16, false, a.outer, a.C, a.inner, a.x_sc, 0);
-  // a lane's neighbours hold a whole block of 32 in every register form but the widest planar one in float
-  if (a.codes && (p.slabs == 0 || (!rows && !a16 && a.C > 2048))) {   // the checkpoint of x as a pass of its own
+  const bool one = !rows && norm_one_pixel(a, false);
+  const NormPlan p = norm_plan(rows || one, a16, false, a.outer, a.C, a.inner, a.x_sc, 0);
+  if (a.codes && (p.slabs == 0 || one)) {   // the checkpoint of x as a pass of its own
     Q8PackArgs q;
     q.x = a.x; q.codes = a.codes; q.exps = a.exps; q.nblk = a.nblk;
     q.outer = rows ? 1 : a.outer; q.rows = rows ? a.outer : a.C; q.cols = rows ? a.C : a.inner;
@@ -674,6 +736,7 @@ int csn_launch_norm_fwd(const NormArgs& a0, int rows, int a16, int fmt, void* st
     if (e != 0) return e;
     a.codes = nullptr;
   }
+  if (one) rows = 1;
 #ifndef CSN_EMU_SEQ
   if (p.slabs > 0) return norm_fast(a, p, rows, a16, a.codes ? fmt : NORM_X, false, stream);
 #endif
@@ -692,15 +755,16 @@ static int norm_bwd(const NormArgs& a, void* stream) {
 
 int csn_launch_norm_bwd(const NormArgs& a0, int rows, int a16, int fmt, void* stream) {
   NormArgs a = a0;
+  if (!rows && norm_one_pixel(a, true)) rows = 1;
   const NormPlan p = norm_plan(rows, a16, true, a.outer, a.C, a.inner, a.x_sc, a.dy_sc);
 #ifndef CSN_EMU_SEQ
   if (p.slabs > 0) {
     if (!a.dweight && !a.dbias) a.partial = nullptr;
     const int e = norm_fast(a, p, rows, a16, a.x ? NORM_X : fmt, true, stream);
     if (e != 0 || !a.partial || p.slabs == 1) return e;
-    a.slabs = (int32_t)p.slabs;
-    CSN_LAUNCH(norm_reduce_kernel, dim3((unsigned)((2 * a.C + 63) / 64)), dim3(1024), 1024 * sizeof(double), stream, a);
-    return (int)hipGetLastError();
+    SlabSumArgs r;
+    r.partial = a.partial; r.out0 = a.dweight; r.out1 = a.dbias; r.n0 = a.C; r.n = 2 * a.C; r.slabs = (int32_t)p.slabs;
+    return csn_launch_slab_sum(r, stream);
   }
 #endif
   if (fmt == Q8_INT8) {
@@ -712,6 +776,7 @@ int csn_launch_norm_bwd(const NormArgs& a0, int rows, int a16, int fmt, void* st
 }
 
 int64_t csn_norm_partial_floats(int rows, int a16, int64_t outer, int64_t C, int64_t inner) {
-  const int64_t slabs = norm_plan(rows, a16, true, outer, C, inner, 0, 0).slabs;   // (strides only ever lower the count)
+  // (strides decide between the forms, never for more slabs; maps of one pixel may run as rows)
+  const int64_t slabs = norm_plan(rows || inner == 1, a16, true, outer, C, inner, 0, 0).slabs;
   return slabs > 1 ? slabs * 2 * C : 0;
 }

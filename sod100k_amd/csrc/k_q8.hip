@@ -17,10 +17,9 @@ int csn_launch_q8_unpack(const Q8UnpackArgs&, int, int, void*) { return -1; }
 
 #define Q8_VECS 2    // 16-byte vectors of the tensor per piece
 
-template <typename AT, int FMT>
+template <typename AT, int FMT, bool W>
 __global__ __launch_bounds__(CSN_BLOCK) void q8_pack_kernel(Q8PackArgs a) {
   constexpr int E = VecIo<AT>::E, L = Q8_VECS * E;   // elements of a piece; 32 / L lanes hold a block
-  const bool wide = a.cols >= L;
   const int64_t stride = (int64_t)gridDim.x * CSN_BLOCK;
   for (int64_t i = (int64_t)blockIdx.x * CSN_BLOCK + threadIdx.x; i < a.items; i += stride) {
     // (a wave's pieces of one block never part: items is a multiple of 32 / L lanes)
@@ -41,12 +40,12 @@ __global__ __launch_bounds__(CSN_BLOCK) void q8_pack_kernel(Q8PackArgs a) {
     const AT* x = reinterpret_cast<const AT*>(a.x) + o * a.so + (row - o * a.rows) * a.sr + pos;
     VecIo<AT> v[Q8_VECS];
 #pragma unroll
-    for (int q = 0; q < Q8_VECS; ++q) vec_load(v[q], x + q * E, n - q * E, wide);
+    for (int q = 0; q < Q8_VECS; ++q) vec_load<W>(v[q], x + q * E, n - q * E);
     float f[L];
 #pragma unroll
     for (int q = 0; q < Q8_VECS; ++q) {
       float g[E];
-      vec_end(v[q], n - q * E, wide);
+      vec_end<W>(v[q], n - q * E);
       v[q].get(g);
 #pragma unroll
       for (int j = 0; j < E; ++j) f[q * E + j] = g[j];
@@ -75,10 +74,9 @@ __global__ __launch_bounds__(CSN_BLOCK) void q8_pack_kernel(Q8PackArgs a) {
   }
 }
 
-template <typename AT, int FMT>
+template <typename AT, int FMT, bool W>
 __global__ __launch_bounds__(CSN_BLOCK) void q8_unpack_kernel(Q8UnpackArgs a) {
   constexpr int E = VecIo<AT>::E, L = Q8_VECS * E;
-  const bool wide = a.cols >= L;
   const int64_t stride = (int64_t)gridDim.x * CSN_BLOCK;
   for (int64_t i = (int64_t)blockIdx.x * CSN_BLOCK + threadIdx.x; i < a.items; i += stride) {
     int64_t row = 0, pos = i * L;
@@ -103,8 +101,8 @@ __global__ __launch_bounds__(CSN_BLOCK) void q8_unpack_kernel(Q8UnpackArgs a) {
     } else {
 #pragma unroll
       for (int q = 0; q < Q8_VECS; ++q) {
-        code_load<E>(v[q], c + q * E, n - q * E, wide);
-        code_end<E>(v[q], n - q * E, wide);
+        code_load<W, E>(v[q], c + q * E, n - q * E);
+        code_end<W, E>(v[q], n - q * E);
       }
     }
     const float sc = q8_scale(a.exps[i / (32 / L)]);
@@ -123,6 +121,21 @@ static unsigned q8_grid(int64_t items) {
   return (unsigned)(g < 65536 ? g : 65536);
 }
 
+template <typename AT, int FMT>
+static int q8_pack_run(const Q8PackArgs& a, void* stream) {
+  const dim3 g(q8_grid(a.items)), b(CSN_BLOCK);
+  if (a.cols >= VecIo<AT>::E) CSN_LAUNCH((q8_pack_kernel<AT, FMT, true>), g, b, 0, stream, a);
+  else CSN_LAUNCH((q8_pack_kernel<AT, FMT, false>), g, b, 0, stream, a);
+  return (int)hipGetLastError();
+}
+template <typename AT, int FMT>
+static int q8_unpack_run(const Q8UnpackArgs& a, void* stream) {
+  const dim3 g(q8_grid(a.items)), b(CSN_BLOCK);
+  if (a.cols >= VecIo<AT>::E) CSN_LAUNCH((q8_unpack_kernel<AT, FMT, true>), g, b, 0, stream, a);
+  else CSN_LAUNCH((q8_unpack_kernel<AT, FMT, false>), g, b, 0, stream, a);
+  return (int)hipGetLastError();
+}
+
 int csn_launch_q8_pack(const Q8PackArgs& a0, int a16, int fmt, void* stream) {
   Q8PackArgs a = a0;
   if (a.outer * a.rows * a.cols <= 0) return 0;
@@ -134,15 +147,8 @@ int csn_launch_q8_pack(const Q8PackArgs& a0, int a16, int fmt, void* stream) {
   a.nblk = (a.cols + 31) / 32;
   a.per_row = a.nblk * (a16 ? 2 : 4);
   a.items = a.nrows * a.per_row;
-  const dim3 g(q8_grid(a.items)), b(CSN_BLOCK);
-  if (a16) {
-    if (fmt == Q8_INT8) CSN_LAUNCH((q8_pack_kernel<csn_bf16, Q8_INT8>), g, b, 0, stream, a);
-    else CSN_LAUNCH((q8_pack_kernel<csn_bf16, Q8_E4M3>), g, b, 0, stream, a);
-  } else {
-    if (fmt == Q8_INT8) CSN_LAUNCH((q8_pack_kernel<float, Q8_INT8>), g, b, 0, stream, a);
-    else CSN_LAUNCH((q8_pack_kernel<float, Q8_E4M3>), g, b, 0, stream, a);
-  }
-  return (int)hipGetLastError();
+  if (a16) return fmt == Q8_INT8 ? q8_pack_run<csn_bf16, Q8_INT8>(a, stream) : q8_pack_run<csn_bf16, Q8_E4M3>(a, stream);
+  return fmt == Q8_INT8 ? q8_pack_run<float, Q8_INT8>(a, stream) : q8_pack_run<float, Q8_E4M3>(a, stream);
 }
 
 int csn_launch_q8_unpack(const Q8UnpackArgs& a0, int a16, int fmt, void* stream) {
@@ -152,14 +158,7 @@ int csn_launch_q8_unpack(const Q8UnpackArgs& a0, int a16, int fmt, void* stream)
   a.nblk = (a.cols + 31) / 32;
   a.per_row = a.nblk * (a16 ? 2 : 4);
   a.items = a.rows * a.per_row;
-  const dim3 g(q8_grid(a.items)), b(CSN_BLOCK);
-  if (a16) {
-    if (fmt == Q8_INT8) CSN_LAUNCH((q8_unpack_kernel<csn_bf16, Q8_INT8>), g, b, 0, stream, a);
-    else CSN_LAUNCH((q8_unpack_kernel<csn_bf16, Q8_E4M3>), g, b, 0, stream, a);
-  } else {
-    if (fmt == Q8_INT8) CSN_LAUNCH((q8_unpack_kernel<float, Q8_INT8>), g, b, 0, stream, a);
-    else CSN_LAUNCH((q8_unpack_kernel<float, Q8_E4M3>), g, b, 0, stream, a);
-  }
-  return (int)hipGetLastError();
+  if (a16) return fmt == Q8_INT8 ? q8_unpack_run<csn_bf16, Q8_INT8>(a, stream) : q8_unpack_run<csn_bf16, Q8_E4M3>(a, stream);
+  return fmt == Q8_INT8 ? q8_unpack_run<float, Q8_INT8>(a, stream) : q8_unpack_run<float, Q8_E4M3>(a, stream);
 }
 #endif  // CSN_EMU_SEQ

@@ -17,6 +17,7 @@
 // Few tiles and many tokens are the usual case (the channels of a map against its pixels), so the tokens are cut into slabs whose
 // partial tiles a second kernel adds in order.
 #include "q8_core.h"
+#include "slab_sum.h"
 #include "train_ops.h"
 
 #ifdef CSN_EMU_SEQ
@@ -316,7 +317,7 @@ __global__ __launch_bounds__(CSN_BLOCK) void q8_wgrad_kernel(Q8WgradArgs a) {
     if (s + 1 < s1) store(sm + cur * BUF);
   }
 
-  float* out = a.slabs > 1 ? a.partial + (int64_t)slab * a.cout * a.cin : a.dweight;
+  float* out = a.slabs > 1 ? a.partial + (int64_t)slab * a.cout * (a.cin + 1) : a.dweight;
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -346,30 +347,8 @@ __global__ __launch_bounds__(CSN_BLOCK) void q8_wgrad_kernel(Q8WgradArgs a) {
       float v = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) v += sb[tid * 8 + j];
-      (a.slabs > 1 ? a.partial + (int64_t)a.slabs * a.cout * a.cin + (int64_t)slab * a.cout : a.dbias)[o0 + tid] = v;
+      (a.slabs > 1 ? out + a.cout * a.cin : a.dbias)[o0 + tid] = v;   // (behind the slab's dW)
     }
-  }
-}
-
-// the sum over the slabs in order: 64 consecutive elements per block, wave w adds slabs w, w + 16, ...
-__global__ __launch_bounds__(1024) void q8_wgrad_reduce_kernel(Q8WgradArgs a) {
-  CSN_DYN_SMEM(double, sd);   // [16][64]
-  const int64_t n = a.cout * a.cin, nb = a.dbias ? a.cout : 0;
-  const int64_t e = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-  const int w = threadIdx.x >> 6;
-  const bool isb = e >= n;
-  double v = 0.0;
-  if (e < n + nb) {
-    const float* p = isb ? a.partial + (int64_t)a.slabs * n + (e - n) : a.partial + e;
-    const int64_t st = isb ? a.cout : n;
-#pragma unroll 4
-    for (int s = w; s < a.slabs; s += 16) v += p[(int64_t)s * st];
-  }
-  sd[w * 64 + (threadIdx.x & 63)] = v;
-  __syncthreads();
-  if (w == 0 && e < n + nb) {
-    for (int q = 1; q < 16; ++q) v += sd[q * 64 + (threadIdx.x & 63)];
-    (isb ? a.dbias[e - n] : a.dweight[e]) = (float)v;
   }
 }
 
@@ -415,8 +394,11 @@ static int q8_wgrad_run(const Q8WgradArgs& a, void* stream) {
   const int total = a.mtiles * a.ntiles * a.slabs;
   CSN_LAUNCH((q8_wgrad_kernel<AT, FMT, ROWS, TM, TN>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(CSN_BLOCK), smem, stream, a);
   if (a.slabs > 1) {
-    const int64_t n = a.cout * a.cin + (a.dbias ? a.cout : 0);
-    CSN_LAUNCH(q8_wgrad_reduce_kernel, dim3((unsigned)((n + 63) / 64)), dim3(1024), 1024 * sizeof(double), stream, a);
+    const int e = (int)hipGetLastError();
+    if (e != 0) return e;
+    SlabSumArgs r;
+    r.partial = a.partial; r.out0 = a.dweight; r.out1 = a.dbias; r.n0 = a.cout * a.cin; r.n = r.n0 + a.cout; r.slabs = a.slabs;
+    return csn_launch_slab_sum(r, stream);
   }
   return (int)hipGetLastError();
 }

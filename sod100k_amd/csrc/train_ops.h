@@ -57,7 +57,7 @@ struct Q8WgradArgs {
   const uint8_t* exps;
   float* dweight;
   float* dbias;
-  float* partial;           // [slabs][cout][cin], then [slabs][cout]
+  float* partial;           // [slabs][cout * cin + cout]
   int64_t outer, inner, cin, cout;
   int64_t dy_so, dy_sc;
   int64_t nblk;             // checkpoint blocks of a plane / row
