@@ -372,6 +372,7 @@ __device__ __forceinline__ void norm_planar_sum(float (&v)[N][E], float* sm, int
       if (PX <= 4) v[i][j] += csn_lane_xor_f32<4>(v[i][j]);
       if (PX <= 2) v[i][j] += csn_lane_xor_f32<2>(v[i][j]);
     }
+  if (W == 1) return;
   float* b = sm + turn * (W * N * TP);
   turn ^= 1;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, px = lane % PX;
@@ -515,46 +516,63 @@ __global__ __launch_bounds__(T) void norm_planar_bwd_kernel(NormArgs a) {
   const unsigned xlane = (unsigned)cg * (unsigned)a.x_sc + px * E, dlane = (unsigned)cg * (unsigned)a.dy_sc + px * E;
   const unsigned ylane = (unsigned)cg * (unsigned)P + px * E;
   int turn = 0;
-  for (int it = blockIdx.x; it < a.items; it += gridDim.x) {
+  NormIn<AT, E, SRC> nx[NC];
+  VecIo<AT, E> nd[NC];
+  VecIo<float> nm, nr;   // mean, rstd of the lane's pixels
+  auto load = [&](int it) {
     const int o = it / a.tiles, t0 = (it - o * a.tiles) * TP;
     const int n = P - t0 - px * E;
     const int64_t row0 = (int64_t)o * C;
     const AT* x = reinterpret_cast<const AT*>(a.x) + o * a.x_so;
     const AT* dy = reinterpret_cast<const AT*>(a.dy) + o * a.dy_so;
     const int tb = t0 - vec_back(n > 0 ? n : E, E);
-    const unsigned xoff = (xlane + tb) * ES, doff = (dlane + tb) * ES, coff = ylane + tb, yoff = (ylane + t0) * ES;
+    const unsigned xoff = (xlane + tb) * ES, doff = (dlane + tb) * ES, coff = ylane + tb;
     const unsigned eoff = (unsigned)cg * (unsigned)a.nblk + ((t0 + px * E) >> 5);
-    NormIn<AT, E, SRC> rx[NC];
-    VecIo<AT, E> rd[NC];
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       const int m = cg + CG * k < C ? n : 0;
       if constexpr (SRC == NORM_X) {
-        norm_load(rx[k].v, x + (int64_t)(CG * k) * a.x_sc, xoff, m);
+        norm_load(nx[k].v, x + (int64_t)(CG * k) * a.x_sc, xoff, m);
       } else {
-        rx[k].c.zero();
-        rx[k].e = 127;
+        nx[k].c.zero();
+        nx[k].e = 127;
         if (m > 0) {
-          rx[k].c.load(norm_at(a.codes_in + (row0 + CG * k) * P, coff));
-          rx[k].e = *norm_at(a.exps_in + (row0 + CG * k) * a.nblk, eoff);
+          nx[k].c.load(norm_at(a.codes_in + (row0 + CG * k) * P, coff));
+          nx[k].e = *norm_at(a.exps_in + (row0 + CG * k) * a.nblk, eoff);
         }
       }
-      norm_load(rd[k], dy + (int64_t)(CG * k) * a.dy_sc, doff, m);
+      norm_load(nd[k], dy + (int64_t)(CG * k) * a.dy_sc, doff, m);
     }
-    float mean[E], rstd[E], s[2][E];
     const int64_t st = (int64_t)o * P + t0 + px * E;
+    vec_load<true>(nm, a.mean + st, n);
+    vec_load<true>(nr, a.rstd + st, n);
+  };
+  if ((int)blockIdx.x < a.items) load(blockIdx.x);
+  for (int it = blockIdx.x; it < a.items; it += gridDim.x) {
+    const int o = it / a.tiles, t0 = (it - o * a.tiles) * TP;
+    const int n = P - t0 - px * E;
+    const int64_t row0 = (int64_t)o * C;
+    const unsigned yoff = (ylane + t0) * ES;
+    NormIn<AT, E, SRC> rx[NC];
+    VecIo<AT, E> rd[NC];
+    VecIo<float> cm = nm, cr = nr;
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      mean[j] = j < n ? a.mean[st + j] : 0.f;
-      rstd[j] = j < n ? a.rstd[st + j] : 0.f;
-      s[0][j] = s[1][j] = 0.f;
-    }
-    if (t0 + TP > P)
+    for (int k = 0; k < NC; ++k) { rx[k] = nx[k]; rd[k] = nd[k]; }
+    if (it + (int)gridDim.x < a.items) load(it + gridDim.x);   // (in flight while this tile is worked on)
+    if (t0 + TP > P) {   // (the image's last tile, one branch for all channels: the sums below stay one straight block)
+      vec_end<true>(cm, n);
+      vec_end<true>(cr, n);
 #pragma unroll
       for (int k = 0; k < NC; ++k) {
         rx[k].template end<true>(n);
         vec_end<true>(rd[k], n);
       }
+    }
+    float mean[E], rstd[E], s[2][E];
+    cm.get(mean);
+    cr.get(rstd);
+#pragma unroll
+    for (int j = 0; j < E; ++j) s[0][j] = s[1][j] = 0.f;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       float f[E], d[E];
@@ -605,13 +623,10 @@ __global__ __launch_bounds__(T) void norm_planar_bwd_kernel(NormArgs a) {
   }
 }
 
-// blocks of a persistent launch: the chip's 256 CUs full of waves
-#ifdef NORM_TUNE
-#include <cstdlib>
-static int64_t norm_blocks(int threads) { const char* e = std::getenv("NORM_W"); return 256 * (int64_t)((e ? std::atoi(e) : 2048) / threads); }
-#else
-static int64_t norm_blocks(int threads) { return 256 * (int64_t)(2048 / threads); }
-#endif
+// Blocks of a persistent launch on 256 CUs: 2048 threads each (all their waves) for the forward, 1024 for the backward, whose registers hold the
+// next token as well and whose blocks leave a slab of weight gradients each (32x256x88x88 bf16: 94.0 against 96.5 us, 32x256x56x56
+// float 62.6 against 67.2 us with the sums of the slabs)
+static int64_t norm_blocks(int threads, bool bwd) { return 256 * (int64_t)std::max((bwd ? 1024 : 2048) / threads, 1); }
 
 // The register forms: which one takes a case, what its grid is.  slabs = 0: none.
 struct NormPlan { int G, NV; int T, PX, NC; int64_t slabs, tiles, items; };
@@ -624,22 +639,30 @@ static NormPlan norm_plan(int rows, int a16, bool bwd, int64_t outer, int64_t C,
     p.NV = C <= (int64_t)p.G * 8 ? 1 : 2;
     p.T = std::max(p.G, CSN_BLOCK);
     const int r = p.T / p.G;
-    p.slabs = std::min(norm_blocks(p.T), (outer + r - 1) / r);
+    p.slabs = std::min(norm_blocks(p.T, bwd), (outer + r - 1) / r);
     return p;
   }
   if (C > 2048 || inner < NORM_PE) return p;
-  // 16 lanes of 8 bytes (bfloat16) or 8 of 16 (float) read 128 bytes of a channel; wider tokens than their threads can hold narrow
-  // the tile.  The forward holds one piece per channel and lane, the backward two and two sums
-  p.T = C <= 128 ? 256 : C <= 256 ? 512 : 1024;
-  p.PX = a16 ? (C <= 512 ? 16 : C <= 1024 || !bwd ? 8 : 4) : (C <= 512 ? 8 : !bwd ? 8 : C <= 1024 ? 4 : 2);
+  // The forward does best with the most channels per lane that fit its registers and 16 lanes (128 / 256 bytes of a channel) across the
+  // pixels: 16 channels 46 us, 8 channels 52 us (32x256x88x88 bf16), 36 against 50 us (16x512x44x44 float with a checkpoint).  The backward
+  // holds two tensors, the next tile of both and two sums per channel: 8 channels (4 in float and in blocks of 1024 threads, whose
+  // registers are half as many) 94 us, 16 channels 120 us.  Wider tokens than that narrow the tile.
+  if (!bwd) {
+    p.T = C <= 64 ? 128 : C <= 128 ? 128 : C <= 256 ? 256 : C <= 512 ? 512 : 1024;
+    p.PX = C <= 1024 ? 16 : 8;
+    p.NC = C <= 64 ? 8 : 16;
+  } else {
+    p.T = C <= 64 ? 128 : C <= 128 ? 256 : C <= 256 ? 512 : 1024;
+    p.PX = C <= 128 ? 16 : C <= 256 ? (a16 ? 16 : 8) : C <= 512 ? 8 : C <= 1024 ? 4 : 2;
+    p.NC = C <= 128 || (C <= 256 && a16) ? 8 : 4;
+  }
   const int cg = p.T / p.PX;
-  p.NC = C <= 4 * cg ? 4 : C <= 8 * cg ? 8 : 16;
   const int64_t tile = (int64_t)p.PX * NORM_PE, lim = (int64_t)1 << 29;
   p.tiles = (inner + tile - 1) / tile;
   p.items = outer * p.tiles;
   // 32-bit byte offsets of a lane and 32-bit item counts
   if (inner > lim || p.items > lim || cg * std::max(inner, std::max(x_sc, dy_sc)) + inner + tile > lim) { p.slabs = 0; return p; }
-  p.slabs = std::min(norm_blocks(p.T), p.items);
+  p.slabs = std::min(norm_blocks(p.T, bwd), p.items);
   return p;
 }
 
@@ -675,25 +698,20 @@ static int norm_planar_bwd(const NormArgs& a, void* stream) {
   CSN_LAUNCH((norm_planar_bwd_kernel<AT, T, PX, NC, CK>), dim3((unsigned)a.slabs), dim3(T), sm, stream, a);
   return (int)hipGetLastError();
 }
-template <typename AT, int T, int PX, int NC, int CK>
-static int norm_planar_go(const NormArgs& a, bool bwd, void* stream) {
-  return bwd ? norm_planar_bwd<AT, T, PX, NC, CK>(a, stream) : norm_planar_fwd<AT, T, PX, NC, CK>(a, stream);
-}
 template <typename AT, int CK>
 static int norm_planar_run(const NormArgs& a, const NormPlan& p, bool bwd, void* stream) {
-  if constexpr (sizeof(AT) == 2) {
-    if (p.T == 256) return p.NC == 4 ? norm_planar_go<AT, 256, 16, 4, CK>(a, bwd, stream) : norm_planar_go<AT, 256, 16, 8, CK>(a, bwd, stream);
-    if (p.T == 512) return norm_planar_go<AT, 512, 16, 8, CK>(a, bwd, stream);
-    if (p.PX == 16) return norm_planar_go<AT, 1024, 16, 8, CK>(a, bwd, stream);
-    if (p.PX == 8 && p.NC == 8) return norm_planar_go<AT, 1024, 8, 8, CK>(a, bwd, stream);
-    return bwd ? norm_planar_bwd<AT, 1024, 4, 8, CK>(a, stream) : norm_planar_fwd<AT, 1024, 8, 16, CK>(a, stream);
-  } else {
-    if (p.T == 256) return norm_planar_go<AT, 256, 8, 4, CK>(a, bwd, stream);
-    if (p.T == 512) return norm_planar_go<AT, 512, 8, 4, CK>(a, bwd, stream);
-    if (p.PX == 8 && p.NC == 4) return norm_planar_go<AT, 1024, 8, 4, CK>(a, bwd, stream);
-    if (p.PX == 8) return p.NC == 8 ? norm_planar_fwd<AT, 1024, 8, 8, CK>(a, stream) : norm_planar_fwd<AT, 1024, 8, 16, CK>(a, stream);
-    return p.PX == 4 ? norm_planar_bwd<AT, 1024, 4, 4, CK>(a, stream) : norm_planar_bwd<AT, 1024, 2, 4, CK>(a, stream);
+  if (!bwd) {
+    if (p.NC == 8) return norm_planar_fwd<AT, 128, 16, 8, CK>(a, stream);
+    if (p.T == 128) return norm_planar_fwd<AT, 128, 16, 16, CK>(a, stream);
+    if (p.T == 256) return norm_planar_fwd<AT, 256, 16, 16, CK>(a, stream);
+    if (p.T == 512) return norm_planar_fwd<AT, 512, 16, 16, CK>(a, stream);
+    return p.PX == 16 ? norm_planar_fwd<AT, 1024, 16, 16, CK>(a, stream) : norm_planar_fwd<AT, 1024, 8, 16, CK>(a, stream);
   }
+  if (p.T == 128) return norm_planar_bwd<AT, 128, 16, 8, CK>(a, stream);
+  if (p.T == 256) return norm_planar_bwd<AT, 256, 16, 8, CK>(a, stream);
+  if (p.T == 512) return norm_planar_bwd<AT, 512, sizeof(AT) == 2 ? 16 : 8, sizeof(AT) == 2 ? 8 : 4, CK>(a, stream);
+  if (p.PX == 8) return norm_planar_bwd<AT, 1024, 8, 4, CK>(a, stream);
+  return p.PX == 4 ? norm_planar_bwd<AT, 1024, 4, 4, CK>(a, stream) : norm_planar_bwd<AT, 1024, 2, 4, CK>(a, stream);
 }
 template <int CK>
 static int norm_fast(const NormArgs& a, const NormPlan& p, int rows, int a16, bool bwd, void* stream) {
