@@ -203,6 +203,18 @@ int csn_plan_enable_training(csn_plan* plan);
 int csn_backward(csn_plan* plan, const float* x, const float* dy, void* workspace, const float* arena, float* grad,
                  int64_t arena_floats, const float* flop_w, float pen_scale, void* stream);
 
+/* 8-bit checkpoint of a train-mode forward (format: csn_q8_pack below): everything csn_backward reads of it in the workspace and the plan -- stored
+ * activations, raw convolution outputs and pooled inputs as 8-bit checkpoints, one row per plane; the |GAP| tables, the bfloat16 copy of the
+ * images and the packed tables as they are.  Taken after a csn_forward_train and before anything else writes the workspace, it lets
+ * further forwards run on the plan before the first one's backward: restore it and call csn_backward with that forward's x (and
+ * flop_w).  The gradients are those of the checkpoint's values.  Parameters must not change in between, as for any backward.
+ * `checkpoint` is 256-byte aligned; launches on `stream`, no allocation. */
+size_t csn_plan_checkpoint_bytes(const csn_plan* plan);   /* 0 before csn_plan_enable_training */
+int csn_plan_checkpoint_save(csn_plan* plan, const void* workspace, int32_t format, void* checkpoint, size_t checkpoint_bytes,
+                             void* stream);
+int csn_plan_checkpoint_restore(csn_plan* plan, void* workspace, int32_t format, const void* checkpoint, size_t checkpoint_bytes,
+                                void* stream);
+
 /* Caller-side training maths on flat device buffers.
  * csn_bce_with_logits: *loss (device, fp64, NOT cleared) += mean BCE-with-logits (train.py:209), dy = d mean / d y.
  * csn_adam_step: torch.optim.Adam with L2 weight decay folded into the gradient (train.py:108-123); wd[i] is the

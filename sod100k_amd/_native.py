@@ -309,6 +309,12 @@ def bind(lib: C.CDLL) -> C.CDLL:
     p, i32, i64 = C.c_void_p, C.c_int32, C.c_int64
     lib.csn_q8_pack.restype = C.c_int
     lib.csn_q8_pack.argtypes = [p, i32, i64, i64, i64, i64, i64, i32, p, p, p]
+    lib.csn_plan_checkpoint_bytes.restype = C.c_size_t
+    lib.csn_plan_checkpoint_bytes.argtypes = [p]
+    lib.csn_plan_checkpoint_save.restype = C.c_int
+    lib.csn_plan_checkpoint_save.argtypes = [p, p, i32, p, C.c_size_t, p]
+    lib.csn_plan_checkpoint_restore.restype = C.c_int
+    lib.csn_plan_checkpoint_restore.argtypes = [p, p, i32, p, C.c_size_t, p]
     lib.csn_q8_unpack.restype = C.c_int
     lib.csn_q8_unpack.argtypes = [p, p, i32, i64, i64, p, i32, p]
     lib.csn_layer_norm_forward.restype = C.c_int
@@ -364,7 +370,8 @@ EXPORTS: Sequence[str] = (
     "csf_head_create", "csf_head_destroy", "csf_head_workspace_bytes", "csf_head_refresh_params", "csf_head_forward",
     "csf_head_stage_info", "csf_head_macs", "csf_bn_act", "csn_build_sources_sha16",
     "csn_q8_pack", "csn_q8_unpack", "csn_layer_norm_forward", "csn_layer_norm_workspace_bytes", "csn_layer_norm_backward",
-    "csn_product_weight_grad_workspace_bytes", "csn_product_weight_grad")
+    "csn_product_weight_grad_workspace_bytes", "csn_product_weight_grad",
+    "csn_plan_checkpoint_bytes", "csn_plan_checkpoint_save", "csn_plan_checkpoint_restore")
 
 _lib: Optional[C.CDLL] = None
 

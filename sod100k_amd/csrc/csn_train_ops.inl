@@ -46,9 +46,77 @@ size_t product_ws(const csn_product_desc* d) {
          sizeof(float);
 }
 
+// What csn_backward reads of a train-mode forward, in a fixed order: q(tensor in the workspace, planes, pixels) for activation-typed
+// tensors -- the stored activations, the raw convolution outputs, pooled inputs -- and r(pointer, bytes) for the rest: the per-image |GAP|
+// tables of the penalty, the bfloat16 copy of the images and the plan's packed tables, whose BatchNorm scale / shift / mean / invstd
+// are the batch's.  (The other workspace regions are scratch of one pass.)
+template <class Q, class R>
+void plan_saved(const csn_plan* P, Q&& q, R&& r) {
+  auto act = [&](int64_t off, int C, int lvl) {
+    if (off >= 0 && C > 0) q(off, (int64_t)P->S * C, (int64_t)(P->H >> lvl) * (P->W >> lvl));
+  };
+  for (int i = 1; i < (int)P->acts.size(); ++i) {
+    if (P->virt_cons[i] < 0) act(P->acts[i].ws_off, P->acts[i].channels, P->acts[i].lvl);
+    act(P->tz_off[i], P->acts[i].channels, P->acts[i].lvl);
+  }
+  for (const UnitPlan& u : P->units)
+    for (int i = 0; i < CSN_MAX_BRANCH; ++i) {
+      act(u.pooled_off[i], u.d.cin[i], u.base_lvl + i);
+      act(u.mp_off[i], u.d.cin[i], u.base_lvl + i + 1);
+      if (u.gap_off[i] >= 0) r(u.gap_off[i], (int64_t)u.d.cout[i] * P->S * (int64_t)sizeof(float));
+    }
+  if (P->act16) r(P->x16_off, (int64_t)P->S * P->acts[0].channels * P->H * P->W * 2);
+  r((int64_t)-1, P->packed_floats * (int64_t)sizeof(float));   // (-1: the packed tables, not a workspace region)
+}
+int64_t plan_saved_bytes(const csn_plan* P) {
+  int64_t n = 0;
+  plan_saved(P, [&](int64_t, int64_t rows, int64_t cols) { n += align_up(rows * cols, 256) + align_up(rows * q8_blocks(cols), 256); },
+             [&](int64_t, int64_t bytes) { n += align_up(bytes, 256); });
+  return n;
+}
+int plan_saved_move(csn_plan* P, char* ws, char* ck, int format, bool pack, void* stream) {
+  std::vector<Q8Seg> qs;
+  std::vector<CopySeg> cs;
+  int64_t at = 0;
+  plan_saved(P,
+             [&](int64_t off, int64_t rows, int64_t cols) {
+               Q8Seg g{};
+               g.x = ws + off; g.rows = rows; g.cols = cols;
+               g.codes = reinterpret_cast<uint8_t*>(ck + at); at += align_up(rows * cols, 256);
+               g.exps = reinterpret_cast<uint8_t*>(ck + at); at += align_up(rows * q8_blocks(cols), 256);
+               qs.push_back(g);
+             },
+             [&](int64_t off, int64_t bytes) {
+               CopySeg g{};
+               uint32_t* t = off >= 0 ? reinterpret_cast<uint32_t*>(ws + off) : reinterpret_cast<uint32_t*>(P->packed);
+               uint32_t* c = reinterpret_cast<uint32_t*>(ck + at);
+               g.src = pack ? t : c; g.dst = pack ? c : t; g.words = bytes / 4; at += align_up(bytes, 256);
+               cs.push_back(g);
+             });
+  LAUNCH_TRY(csn_launch_q8_segments(qs.data(), (int)qs.size(), pack, P->act16 ? 1 : 0, format, stream));
+  LAUNCH_TRY(csn_launch_copy_segments(cs.data(), (int)cs.size(), stream));
+  return CSN_OK;
+}
+
 }  // namespace
 
 extern "C" {
+
+size_t csn_plan_checkpoint_bytes(const csn_plan* P) { return P && P->train ? (size_t)plan_saved_bytes(P) : 0; }
+
+int csn_plan_checkpoint_save(csn_plan* P, const void* workspace, int32_t format, void* checkpoint, size_t checkpoint_bytes, void* stream) {
+  if (!P || !workspace || !checkpoint || ((uintptr_t)checkpoint & 255u) || !format_ok(format)) REFUSE("plan checkpoint: null or misaligned (256 bytes) buffer, unknown format");
+  if (!P->train || !P->bn_tables_train) { g_hip_err = "plan checkpoint: no train-mode forward of a training plan to save"; return CSN_E_STATE; }
+  if (checkpoint_bytes < (size_t)plan_saved_bytes(P)) REFUSE("plan checkpoint: buffer smaller than csn_plan_checkpoint_bytes");
+  return plan_saved_move(P, static_cast<char*>(const_cast<void*>(workspace)), static_cast<char*>(checkpoint), format, true, stream);
+}
+
+int csn_plan_checkpoint_restore(csn_plan* P, void* workspace, int32_t format, const void* checkpoint, size_t checkpoint_bytes, void* stream) {
+  if (!P || !workspace || !checkpoint || ((uintptr_t)checkpoint & 255u) || !format_ok(format)) REFUSE("plan checkpoint: null or misaligned (256 bytes) buffer, unknown format");
+  if (!P->train || !P->bn_tables_train) { g_hip_err = "plan checkpoint: a training plan that has run a forward is needed"; return CSN_E_STATE; }
+  if (checkpoint_bytes < (size_t)plan_saved_bytes(P)) REFUSE("plan checkpoint: buffer smaller than csn_plan_checkpoint_bytes");
+  return plan_saved_move(P, static_cast<char*>(workspace), static_cast<char*>(const_cast<void*>(checkpoint)), format, false, stream);
+}
 
 int csn_q8_pack(const void* x, int32_t dtype, int64_t outer, int64_t rows, int64_t cols, int64_t outer_stride, int64_t row_stride,
                 int32_t format, uint8_t* codes, uint8_t* exponents, void* stream) {

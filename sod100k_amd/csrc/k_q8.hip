@@ -13,13 +13,83 @@
 #ifdef CSN_EMU_SEQ
 int csn_launch_q8_pack(const Q8PackArgs&, int, int, void*) { return -1; }   // (lane exchange: lane-exact mode only)
 int csn_launch_q8_unpack(const Q8UnpackArgs&, int, int, void*) { return -1; }
+int csn_launch_q8_segments(Q8Seg*, int, bool, int, int, void*) { return -1; }
 #else
 
 #define Q8_VECS 2    // 16-byte vectors of the tensor per piece
 
+// piece of n <= L elements at x -> codes at c, and the block's exponent at e from its first lane (32 / L neighbouring lanes, all of
+// them here)
+template <typename AT, int FMT, bool W>
+__device__ __forceinline__ void q8_pack_piece(const AT* x, uint8_t* c, uint8_t* e, int n, bool first) {
+  constexpr int E = VecIo<AT>::E, L = Q8_VECS * E;
+  VecIo<AT> v[Q8_VECS];
+#pragma unroll
+  for (int q = 0; q < Q8_VECS; ++q) vec_load<W>(v[q], x + q * E, n - q * E);
+  float f[L];
+#pragma unroll
+  for (int q = 0; q < Q8_VECS; ++q) {
+    float g[E];
+    vec_end<W>(v[q], n - q * E);
+    v[q].get(g);
+#pragma unroll
+    for (int j = 0; j < E; ++j) f[q * E + j] = g[j];
+  }
+  unsigned w[L / 4];
+  const unsigned s = q8_pack_block<FMT, L>(f, w);
+  if (n >= L) {
+    if (L == 16) {
+      csn_raw16_a1 r;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r.w[j] = w[j % (L / 4)];
+      *reinterpret_cast<csn_raw16_a1*>(c) = r;
+    } else {
+      csn_raw8_a1 r;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) r.w[j] = w[j];
+      *reinterpret_cast<csn_raw8_a1*>(c) = r;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < L; ++j)
+      if (j < n) c[j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
+  }
+  if (first) *e = (uint8_t)s;
+}
+
+template <typename AT, int FMT, bool W>
+__device__ __forceinline__ void q8_unpack_piece(const uint8_t* c, unsigned e, AT* y, int n) {
+  constexpr int E = VecIo<AT>::E, L = Q8_VECS * E;
+  CodeIo<E> v[Q8_VECS];
+  if (n >= L) {
+    if (L == 16) {
+      const csn_raw16_a1 r = *reinterpret_cast<const csn_raw16_a1*>(c);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j / (E / 4) % Q8_VECS].w[j % (E / 4)] = r.w[j];
+    } else {
+      const csn_raw8_a1 r = *reinterpret_cast<const csn_raw8_a1*>(c);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) v[j / (E / 4)].w[j % (E / 4)] = r.w[j];
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < Q8_VECS; ++q) {
+      code_load<W, E>(v[q], c + q * E, n - q * E);
+      code_end<W, E>(v[q], n - q * E);
+    }
+  }
+  const float sc = q8_scale(e);
+#pragma unroll
+  for (int q = 0; q < Q8_VECS; ++q) {
+    float f[E];
+    q8_decode_vec<FMT, E>(v[q].w, sc, f);
+    VecIo<AT>::store(y + q * E, f, n - q * E);
+  }
+}
+
 template <typename AT, int FMT, bool W>
 __global__ __launch_bounds__(CSN_BLOCK) void q8_pack_kernel(Q8PackArgs a) {
-  constexpr int E = VecIo<AT>::E, L = Q8_VECS * E;   // elements of a piece; 32 / L lanes hold a block
+  constexpr int L = Q8_VECS * VecIo<AT>::E;   // elements of a piece; 32 / L lanes hold a block
   const int64_t stride = (int64_t)gridDim.x * CSN_BLOCK;
   for (int64_t i = (int64_t)blockIdx.x * CSN_BLOCK + threadIdx.x; i < a.items; i += stride) {
     // (a wave's pieces of one block never part: items is a multiple of 32 / L lanes)
@@ -36,47 +106,15 @@ __global__ __launch_bounds__(CSN_BLOCK) void q8_pack_kernel(Q8PackArgs a) {
       pos = (i - row * a.per_row) * L;
     }
     const int64_t left = a.cols - pos;
-    const int n = (int)(left < L ? left : L);
     const AT* x = reinterpret_cast<const AT*>(a.x) + o * a.so + (row - o * a.rows) * a.sr + pos;
-    VecIo<AT> v[Q8_VECS];
-#pragma unroll
-    for (int q = 0; q < Q8_VECS; ++q) vec_load<W>(v[q], x + q * E, n - q * E);
-    float f[L];
-#pragma unroll
-    for (int q = 0; q < Q8_VECS; ++q) {
-      float g[E];
-      vec_end<W>(v[q], n - q * E);
-      v[q].get(g);
-#pragma unroll
-      for (int j = 0; j < E; ++j) f[q * E + j] = g[j];
-    }
-    unsigned w[L / 4];
-    const unsigned s = q8_pack_block<FMT, L>(f, w);
-    uint8_t* c = a.codes + row * a.cols + pos;
-    if (n >= L) {
-      if (L == 16) {
-        csn_raw16_a1 r;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) r.w[j] = w[j];
-        *reinterpret_cast<csn_raw16_a1*>(c) = r;
-      } else {
-        csn_raw8_a1 r;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) r.w[j] = w[j];
-        *reinterpret_cast<csn_raw8_a1*>(c) = r;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < L; ++j)
-        if (j < n) c[j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
-    }
-    if ((i & (32 / L - 1)) == 0) a.exps[i / (32 / L)] = (uint8_t)s;   // (a row's pieces are whole blocks, the last one in part empty)
+    // (a row's pieces are whole blocks, the last one in part empty)
+    q8_pack_piece<AT, FMT, W>(x, a.codes + row * a.cols + pos, a.exps + i / (32 / L), (int)(left < L ? left : L), (i & (32 / L - 1)) == 0);
   }
 }
 
 template <typename AT, int FMT, bool W>
 __global__ __launch_bounds__(CSN_BLOCK) void q8_unpack_kernel(Q8UnpackArgs a) {
-  constexpr int E = VecIo<AT>::E, L = Q8_VECS * E;
+  constexpr int L = Q8_VECS * VecIo<AT>::E;
   const int64_t stride = (int64_t)gridDim.x * CSN_BLOCK;
   for (int64_t i = (int64_t)blockIdx.x * CSN_BLOCK + threadIdx.x; i < a.items; i += stride) {
     int64_t row = 0, pos = i * L;
@@ -84,36 +122,36 @@ __global__ __launch_bounds__(CSN_BLOCK) void q8_unpack_kernel(Q8UnpackArgs a) {
       row = a.items <= 0x7fffffff ? (int64_t)((unsigned)i / (unsigned)a.per_row) : i / a.per_row;
       pos = (i - row * a.per_row) * L;
     }
-    const int64_t left = a.cols - pos;
-    const int n = (int)(left < L ? left : L);
-    const uint8_t* c = a.codes + row * a.cols + pos;
-    CodeIo<E> v[Q8_VECS];
-    if (n >= L) {
-      if (L == 16) {
-        const csn_raw16_a1 r = *reinterpret_cast<const csn_raw16_a1*>(c);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j / (E / 4)].w[j % (E / 4)] = r.w[j];
-      } else {
-        const csn_raw8_a1 r = *reinterpret_cast<const csn_raw8_a1*>(c);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) v[j / (E / 4)].w[j % (E / 4)] = r.w[j];
-      }
-    } else {
-#pragma unroll
-      for (int q = 0; q < Q8_VECS; ++q) {
-        code_load<W, E>(v[q], c + q * E, n - q * E);
-        code_end<W, E>(v[q], n - q * E);
-      }
-    }
-    const float sc = q8_scale(a.exps[i / (32 / L)]);
-    AT* y = reinterpret_cast<AT*>(a.y) + row * a.cols + pos;
-#pragma unroll
-    for (int q = 0; q < Q8_VECS; ++q) {
-      float f[E];
-      q8_decode_vec<FMT, E>(v[q].w, sc, f);
-      VecIo<AT>::store(y + q * E, f, n - q * E);
-    }
+    const int64_t left = a.cols - pos, at = row * a.cols + pos;
+    q8_unpack_piece<AT, FMT, W>(a.codes + at, a.exps[i / (32 / L)], reinterpret_cast<AT*>(a.y) + at, (int)(left < L ? left : L));
   }
+}
+
+// Many tensors of one type in one launch (the saved tensors of a plan): a block finds its segment among the launch's by its number
+// and takes Q8_SEG_PIECES pieces of it.
+#define Q8_SEG_PIECES (4 * CSN_BLOCK)
+template <typename AT, int FMT, bool W, bool PACK>
+__device__ __forceinline__ void q8_segment(const Q8Seg& g, int64_t first) {
+  constexpr int L = Q8_VECS * VecIo<AT>::E;
+  for (int r = 0; r < 4; ++r) {
+    const int64_t i = first + r * CSN_BLOCK + threadIdx.x;
+    if (i >= g.items) return;
+    const int64_t row = g.items <= 0x7fffffff ? (int64_t)((unsigned)i / (unsigned)g.per_row) : i / g.per_row;
+    const int64_t pos = (i - row * g.per_row) * L, left = g.cols - pos, at = row * g.cols + pos;
+    const int n = (int)(left < L ? left : L);
+    AT* x = reinterpret_cast<AT*>(g.x) + at;
+    if (PACK) q8_pack_piece<AT, FMT, W>(x, g.codes + at, g.exps + i / (32 / L), n, (i & (32 / L - 1)) == 0);
+    else q8_unpack_piece<AT, FMT, W>(g.codes + at, g.exps[i / (32 / L)], x, n);
+  }
+}
+template <typename AT, int FMT, bool PACK>
+__global__ __launch_bounds__(CSN_BLOCK) void q8_segments_kernel(Q8SegArgs a) {
+  int s = 0;
+  while (s + 1 < a.n && (int)blockIdx.x >= a.seg[s + 1].block0) ++s;
+  const Q8Seg& g = a.seg[s];
+  const int64_t first = (int64_t)((int)blockIdx.x - g.block0) * Q8_SEG_PIECES;
+  if (g.cols >= VecIo<AT>::E) q8_segment<AT, FMT, true, PACK>(g, first);
+  else q8_segment<AT, FMT, false, PACK>(g, first);
 }
 
 static unsigned q8_grid(int64_t items) {
@@ -161,4 +199,63 @@ int csn_launch_q8_unpack(const Q8UnpackArgs& a0, int a16, int fmt, void* stream)
   if (a16) return fmt == Q8_INT8 ? q8_unpack_run<csn_bf16, Q8_INT8>(a, stream) : q8_unpack_run<csn_bf16, Q8_E4M3>(a, stream);
   return fmt == Q8_INT8 ? q8_unpack_run<float, Q8_INT8>(a, stream) : q8_unpack_run<float, Q8_E4M3>(a, stream);
 }
+
+template <typename AT, int FMT>
+static int q8_segments_run(const Q8SegArgs& a, bool pack, unsigned blocks, void* stream) {
+  if (pack) CSN_LAUNCH((q8_segments_kernel<AT, FMT, true>), dim3(blocks), dim3(CSN_BLOCK), 0, stream, a);
+  else CSN_LAUNCH((q8_segments_kernel<AT, FMT, false>), dim3(blocks), dim3(CSN_BLOCK), 0, stream, a);
+  return (int)hipGetLastError();
+}
+int csn_launch_q8_segments(Q8Seg* seg, int n, bool pack, int a16, int fmt, void* stream) {
+  for (int i = 0; i < n;) {
+    Q8SegArgs a;
+    int64_t blocks = 0;
+    for (a.n = 0; i < n && a.n < Q8_MAX_SEGS; ++i) {
+      Q8Seg g = seg[i];
+      if (g.cols % 32 == 0) { g.cols *= g.rows; g.rows = 1; }
+      g.per_row = (g.cols + 31) / 32 * (a16 ? 2 : 4);
+      g.items = g.rows * g.per_row;
+      if (g.items == 0) continue;
+      const int64_t nb = (g.items + Q8_SEG_PIECES - 1) / Q8_SEG_PIECES;
+      if (blocks + nb > 0x7fffffff) { if (a.n == 0) return -1; break; }
+      g.block0 = (int32_t)blocks;
+      blocks += nb;
+      a.seg[a.n++] = g;
+    }
+    if (a.n == 0) break;
+    const int e = fmt == Q8_INT8 ? (a16 ? q8_segments_run<csn_bf16, Q8_INT8>(a, pack, (unsigned)blocks, stream) : q8_segments_run<float, Q8_INT8>(a, pack, (unsigned)blocks, stream))
+                                 : (a16 ? q8_segments_run<csn_bf16, Q8_E4M3>(a, pack, (unsigned)blocks, stream) : q8_segments_run<float, Q8_E4M3>(a, pack, (unsigned)blocks, stream));
+    if (e != 0) return e;
+  }
+  return 0;
+}
 #endif  // CSN_EMU_SEQ
+
+// ---- plain copies of small tensors, many in one launch (multiples of 4 bytes) --------------------------------------------------
+__global__ __launch_bounds__(CSN_BLOCK) void copy_segments_kernel(CopySegArgs a) {
+  int s = 0;
+  while (s + 1 < a.n && (int)blockIdx.x >= a.seg[s + 1].block0) ++s;
+  const CopySeg& g = a.seg[s];
+  const int64_t i0 = (int64_t)((int)blockIdx.x - g.block0) * (4 * CSN_BLOCK) + threadIdx.x;
+  for (int r = 0; r < 4; ++r)
+    if (i0 + r * CSN_BLOCK < g.words) g.dst[i0 + r * CSN_BLOCK] = g.src[i0 + r * CSN_BLOCK];
+}
+int csn_launch_copy_segments(CopySeg* seg, int n, void* stream) {
+  for (int i = 0; i < n;) {
+    CopySegArgs a;
+    int64_t blocks = 0;
+    for (a.n = 0; i < n && a.n < Q8_MAX_SEGS; ++i) {
+      if (seg[i].words == 0) continue;
+      const int64_t nb = (seg[i].words + 4 * CSN_BLOCK - 1) / (4 * CSN_BLOCK);
+      if (blocks + nb > 0x7fffffff) { if (a.n == 0) return -1; break; }
+      seg[i].block0 = (int32_t)blocks;
+      blocks += nb;
+      a.seg[a.n++] = seg[i];
+    }
+    if (a.n == 0) break;
+    CSN_LAUNCH(copy_segments_kernel, dim3((unsigned)blocks), dim3(CSN_BLOCK), 0, stream, a);
+    const int e = (int)hipGetLastError();
+    if (e != 0) return e;
+  }
+  return 0;
+}

@@ -24,6 +24,22 @@ struct Q8UnpackArgs {
 int csn_launch_q8_pack(const Q8PackArgs& a, int a16, int fmt, void* stream);
 int csn_launch_q8_unpack(const Q8UnpackArgs& a, int a16, int fmt, void* stream);
 
+// one tensor among many (dense rows): x <-> codes, exps
+struct Q8Seg {
+  void* x;
+  uint8_t* codes;
+  uint8_t* exps;
+  int64_t rows, cols;
+  int64_t per_row, items;   // (set by the launcher)
+  int32_t block0, pad;
+};
+#define Q8_MAX_SEGS 48      // of a launch: they travel in its arguments
+struct Q8SegArgs { Q8Seg seg[Q8_MAX_SEGS]; int32_t n, pad; };
+int csn_launch_q8_segments(Q8Seg* seg, int n, bool pack, int a16, int fmt, void* stream);
+struct CopySeg { const uint32_t* src; uint32_t* dst; int64_t words; int32_t block0, pad; };
+struct CopySegArgs { CopySeg seg[Q8_MAX_SEGS]; int32_t n, pad; };
+int csn_launch_copy_segments(CopySeg* seg, int n, void* stream);
+
 struct NormArgs {
   const void* x;            // null: the checkpoint below is the input (backward)
   const void* dy;

@@ -180,6 +180,24 @@ class Engine:
                                                 arena.data_ptr(), grad.data_ptr(), grad.numel(), fw,
                                                 float(pen_scale), self._stream()), "csn_backward")
 
+    def checkpoint_save(self, format: int) -> torch.Tensor:
+        """8-bit checkpoint (``_native.Q8_INT8`` / ``Q8_E4M3``) of the last ``forward_train``: what ``backward`` reads of it."""
+        assert self.train, "engine was created without training buffers"
+        n = int(self.lib.csn_plan_checkpoint_bytes(self.plan))
+        buf = torch.empty(n + 255, dtype=torch.uint8, device=self.device)
+        buf = buf[-buf.data_ptr() % 256:][:n]
+        N.check(self.lib, self.lib.csn_plan_checkpoint_save(self.plan, self.workspace.data_ptr(), format, buf.data_ptr(), n,
+                                                            self._stream()), "csn_plan_checkpoint_save")
+        return buf
+
+    def checkpoint_restore(self, buf: torch.Tensor, format: int) -> None:
+        """Put a checkpoint back into the workspace: ``backward`` then belongs to the forward it was taken of."""
+        assert buf.dtype == torch.uint8 and buf.is_contiguous() and buf.device == self.workspace.device
+        if buf.is_cuda:      # (allocated on the stream of the forward that displaced it)
+            buf.record_stream(torch.cuda.current_stream(self.device))
+        N.check(self.lib, self.lib.csn_plan_checkpoint_restore(self.plan, self.workspace.data_ptr(), format, buf.data_ptr(),
+                                                               buf.numel(), self._stream()), "csn_plan_checkpoint_restore")
+
     def profile(self, x: torch.Tensor, iters: int = 10):
         """Mean milliseconds per unit (HIP events on the launch stream), kernel names, algorithmic bytes."""
         y = torch.empty((self.B, 1, self.H, self.W), dtype=torch.float32, device=x.device)

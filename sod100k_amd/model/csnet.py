@@ -18,6 +18,7 @@ import json
 import math
 import os
 import pickle
+import weakref
 from typing import List, Optional, Sequence
 
 import numpy as np
@@ -511,6 +512,17 @@ class CSNet(nn.Module):
         self._train_act_dtype = dtype
         return self
 
+    def set_train_checkpoints(self, format: Optional[str] = "int8"):
+        """Several train-mode forwards before a backward (accumulated gradients, losses over two forwards): a plan keeps one forward's
+        activations, so with "int8" or "e4m3" the next forward first puts the previous one's saved tensors, if its graph is
+        still waiting for its backward, into an 8-bit checkpoint (csn_plan_checkpoint_save; a quarter / half of the fp32 / bf16
+        tensors).  The last forward's own backward is exact, an earlier one's has the gradients of the checkpoint's values; a step
+        with one forward costs nothing.  None (default): a backward after a newer forward raises."""
+        if format not in (None, "int8", "e4m3"):
+            raise ValueError("train checkpoints must be 'int8', 'e4m3' or None")
+        self._train_checkpoints = format
+        return self
+
     def forward(self, x):
         if x.dim() != 4 or x.shape[1] != 3 or x.dtype != torch.float32:
             raise ValueError("expected a float32 tensor of shape B x 3 x H x W")
@@ -560,6 +572,10 @@ class CSNet(nn.Module):
         """(logits, fp64 device scalar penalty SUM) of one train-mode forward; keeps what csn_backward needs."""
         eng = self.engine_for(x, train=with_backward)
         arena = self._arena
+        waiting = eng.waiting() if getattr(eng, "waiting", None) is not None else None
+        eng.waiting = None
+        if waiting is not None and waiting.format is not None:   # (set_train_checkpoints: an earlier forward's graph still lives)
+            waiting.checkpoint = eng.checkpoint_save(waiting.format)
         eng.refresh(arena.flat)                       # weight blocks + PReLU tables; BN tables are rewritten per batch
         units, _, names = self._desc_cache(arena)
         self._flop_tab = self._flop_weight_table(names, units)
@@ -606,6 +622,11 @@ class _CSNetTrainFn(torch.autograd.Function):
         model._want_input_grad = ctx.input_grad
         y, pen = model._train_forward_raw(x, with_backward=True)
         ctx.model, ctx.x = model, x
+        fmt = getattr(model, "_train_checkpoints", None)
+        if fmt is not None:
+            ctx.saved = _SavedForward(model.engine_for(x, train=True), {"int8": N.Q8_INT8, "e4m3": N.Q8_E4M3}[fmt], model._flop_tab)
+        else:
+            ctx.saved = None
         # backward reads z / activations / BN statistics of THIS forward from the plan's workspace: remember which
         # train-mode forward filled it, so that a second forward before this graph's backward is caught
         ctx.generation = model._train_generation
@@ -614,10 +635,13 @@ class _CSNetTrainFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy, dpen):
         model = ctx.model
+        if ctx.saved is not None:
+            return _CSNetTrainFn._backward_saved(ctx, dy, dpen)
         if ctx.generation != model._train_generation:
             raise RuntimeError("CSNet backward after a newer train-mode forward: the plan keeps the activations of the LAST "
                                "forward only (no gradient accumulation over several forwards / combined losses of two "
-                               "forwards); call backward() before the next model(x)")
+                               "forwards); call backward() before the next model(x), or keep 8-bit checkpoints of the waiting "
+                               "forwards: model.set_train_checkpoints()")
         pen_scale = float(dpen) if dpen is not None else 0.0
         if dy is None:
             dy = torch.zeros((ctx.x.shape[0], 1) + tuple(ctx.x.shape[2:]), dtype=torch.float32, device=ctx.x.device)
@@ -631,6 +655,42 @@ class _CSNetTrainFn(torch.autograd.Function):
             o = offs[name]
             grads.append(flat[o:o + p.numel()].view(p.shape) if p.requires_grad else None)
         return (None, dx) + tuple(grads)
+
+
+    @staticmethod
+    def _backward_saved(ctx, dy, dpen):
+        """Backward with set_train_checkpoints: of the tensors in the workspace if this forward's still lie there untouched, else of
+        its checkpoint."""
+        model, s = ctx.model, ctx.saved
+        eng, arena = s.engine, model._arena
+        if eng.waiting is not None and eng.waiting() is s:
+            pass
+        elif s.checkpoint is not None:
+            eng.waiting, waiting = None, eng.waiting() if eng.waiting is not None else None
+            if waiting is not None:                     # the workspace holds another forward that still waits: out of the way
+                waiting.checkpoint = eng.checkpoint_save(waiting.format)
+            eng.checkpoint_restore(s.checkpoint, s.format)
+        else:
+            raise RuntimeError("CSNet backward a second time through one forward: its saved tensors are gone")
+        eng.waiting = None                              # csn_backward writes over them
+        if dy is None:
+            dy = torch.zeros((ctx.x.shape[0], 1) + tuple(ctx.x.shape[2:]), dtype=torch.float32, device=ctx.x.device)
+        flat = torch.zeros(arena.n_param_floats, dtype=torch.float32, device=ctx.x.device)
+        eng.backward(ctx.x.contiguous(), dy.contiguous(), arena.flat, flat, s.flop_tab, float(dpen) if dpen is not None else 0.0)
+        dx = eng.train_probe(0, "grad0") if ctx.input_grad else None
+        model._want_input_grad = False
+        grads = [flat[arena.offsets[n]:arena.offsets[n] + p.numel()].view(p.shape) if p.requires_grad else None
+                 for n, p in model.named_parameters()]
+        return (None, dx) + tuple(grads)
+
+
+class _SavedForward:
+    """A train-mode forward that waits for its backward (set_train_checkpoints): the plan that ran it and, once another forward
+    needed that plan's workspace, its 8-bit checkpoint.  The plan refers to it weakly: a graph that was dropped saves nothing."""
+
+    def __init__(self, engine, format, flop_tab):
+        self.engine, self.format, self.flop_tab, self.checkpoint = engine, format, flop_tab, None
+        engine.waiting = weakref.ref(self)
 
 
 # ---- dynamic weight decay hook (csnet.py:391-410) -----------------------------------------------------------

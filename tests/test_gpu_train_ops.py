@@ -231,3 +231,14 @@ def test_gpu_offsets_beyond_32_bits(lib):
     dW, dB = T.product_weight_grad(lib, y[:, :8], q)
     ref, _ = T.product_weight_grad(lib, dyt[:, :8], qt)
     assert torch.allclose(dW, ref, rtol=1e-5, atol=1e-6)
+
+
+@pytest.mark.parametrize("act_dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("fmt", K.FORMATS)
+def test_gpu_plan_checkpoint(lib, x2_manifest, act_dtype, fmt):
+    K.check_plan_checkpoint(lib, torch.device(DEV), x2_manifest, act_dtype, fmt, B=3, size=64)
+
+
+@pytest.mark.parametrize("act_dtype,fmt", [("fp32", "e4m3"), ("bf16", "int8")])
+def test_gpu_two_forwards_one_backward(lib, x2_manifest, act_dtype, fmt):
+    K.check_two_forwards_one_backward(lib, torch.device(DEV), x2_manifest, act_dtype, fmt, B=2, size=48)

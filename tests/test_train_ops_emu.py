@@ -104,3 +104,35 @@ def test_no_cpu_fallback(lib, monkeypatch):
         T.layer_norm_forward(lib, torch.zeros(2, 4))
     with pytest.raises(RuntimeError, match="ROCm"):
         T.q8_pack(lib, torch.zeros(2, 4))
+
+
+@pytest.mark.parametrize("act_dtype,fmt", [("fp32", "int8"), ("bf16", "e4m3")])
+def test_emu_plan_checkpoint(lib, x2_manifest, act_dtype, fmt):
+    K.check_plan_checkpoint(lib, torch.device("cpu"), x2_manifest, act_dtype, fmt)
+
+
+def test_emu_two_forwards_one_backward(lib, x2_manifest):
+    K.check_two_forwards_one_backward(lib, torch.device("cpu"), x2_manifest, "fp32", "int8", size=16, quick=True)
+
+
+def test_plan_checkpoint_refusals(lib, x2_manifest):
+    import parity_cases as P
+    m, _ = P.make_model(lib, x2_manifest, torch.device("cpu"))
+    m.train()
+    x = torch.zeros(1, 3, 32, 32)
+    eng = m.engine_for(x, train=True)
+    buf = torch.zeros(1 << 26, dtype=torch.uint8)
+    p = buf.data_ptr() + (-buf.data_ptr() % 256)
+    n = lib.csn_plan_checkpoint_bytes(eng.plan)
+    ws = eng.workspace.data_ptr()
+    for call in (lib.csn_plan_checkpoint_save, lib.csn_plan_checkpoint_restore):
+        assert call(eng.plan, ws, 0, p, n, None) == 5                       # no forward yet
+    m._train_forward_raw(x)
+    for call in (lib.csn_plan_checkpoint_save, lib.csn_plan_checkpoint_restore):
+        assert call(None, ws, 0, p, n, None) == 1 and call(eng.plan, None, 0, p, n, None) == 1
+        assert call(eng.plan, ws, 2, p, n, None) == 1 and call(eng.plan, ws, 0, p + 4, n, None) == 1
+        assert call(eng.plan, ws, 0, p, n - 1, None) == 1 and call(eng.plan, ws, 0, None, n, None) == 1
+    ev = m.eval().engine_for(x)
+    assert lib.csn_plan_checkpoint_bytes(ev.plan) == 0
+    with pytest.raises(ValueError):
+        m.set_train_checkpoints("fp4")

@@ -482,3 +482,125 @@ def check_refusals_of_the_abi(lib):
     need = lib.csn_product_weight_grad_workspace_bytes(pdesc())
     if need:
         bad(prod(pdesc(), nws=need - 1), "workspace")
+
+
+# ---- 8-bit checkpoints of whole forwards (CSNet.set_train_checkpoints) -------------------------------------------------------
+def _net(lib, device, manifest, act_dtype, B):
+    import parity_cases as P
+    m, _ = P.make_model(lib, manifest, device)
+    m.set_train_act_dtype(act_dtype)
+    m.train()
+    m.set_batchsize(B)
+    m.clear_flops()
+    m.flops_hook(1.0)
+    return m
+
+
+def check_plan_checkpoint(lib, device, manifest, act_dtype, fmt, B=2, size=32):
+    """save + restore puts the packed values of every stored activation and raw convolution output where the tensors were, and the
+    backward needs nothing else: with the whole workspace overwritten in between it gives the same bits."""
+    from oracle import inputs as I
+    m = _net(lib, device, manifest, act_dtype, B)
+    f = {"int8": N.Q8_INT8, "e4m3": N.Q8_E4M3}[fmt]
+    x = torch.from_numpy(I.randn_batch(31, B, size, size)).to(device)
+    y, _ = m._train_forward_raw(x)
+    dy = gradient(tuple(y.shape), torch.float32, 1, device)
+    eng = m.engine_for(x, train=True)
+    acts = [i for i in range(1, eng.n_acts)]
+    before = {}
+    for i in acts:
+        for what in ("act", "z"):
+            try:
+                before[i, what] = eng.train_probe(i, what)
+            except ValueError:
+                pass
+    buf = eng.checkpoint_save(f)
+    small = sum(t.numel() for t in before.values())
+    assert buf.numel() < 2.2 * small + (1 << 24)              # one byte an element (pooled copies included) + the packed tables
+    eng.checkpoint_restore(buf, f)
+    changed = 0
+    for (i, what), t in before.items():
+        q = T.q8_pack(m._lib or N.load(), t, fmt, start_dim=2)
+        v, now = T.q8_unpack(m._lib or N.load(), q), eng.train_probe(i, what)
+        if torch.equal(now, t) and not torch.equal(v, t):
+            assert what == "act"                              # (an activation that its consumer forms on load is not stored)
+            continue
+        changed += 1
+        assert same(now.cpu(), v.cpu())
+    assert changed > 0.6 * len(before)
+    g1 = m._train_backward_raw(x, dy, 0.7).clone()
+    eng.workspace.fill_(255)                                   # NaN in every type
+    eng.checkpoint_restore(buf, f)
+    g2 = m._train_backward_raw(x, dy, 0.7)
+    assert bool(torch.isfinite(g2).all()) and torch.equal(g1, g2)
+    return g1
+
+
+def check_two_forwards_one_backward(lib, device, manifest, act_dtype, fmt, B=2, size=32, quick=False):
+    """A loss over two forwards: the newer one's gradients are exact, the older one's those of its checkpoint, whichever goes first;
+    a lone forward is not touched.  quick: the two backwards in autograd's order alone."""
+    from oracle import inputs as I
+    xs = [torch.from_numpy(I.randn_batch(s, B, size, size)).to(device) for s in (31, 32)]
+    f = {"int8": N.Q8_INT8, "e4m3": N.Q8_E4M3}[fmt]
+
+    def lone(x, through_checkpoint):
+        m = _net(lib, device, manifest, act_dtype, B)
+        y, _ = m._train_forward_raw(x)
+        if through_checkpoint:
+            eng = m.engine_for(x, train=True)
+            eng.checkpoint_restore(eng.checkpoint_save(f), f)
+        return m._train_backward_raw(x, gradient(tuple(y.shape), torch.float32, 1, device), 0.0).clone()
+    ck0, exact1 = lone(xs[0], True), lone(xs[1], False)
+
+    def flat(m):
+        out = torch.zeros_like(ck0)
+        for n, p in m.named_parameters():
+            o = m._arena.offsets[n]
+            out[o:o + p.numel()] = p.grad.reshape(-1)
+        return out
+
+    def fresh():
+        m = _net(lib, device, manifest, act_dtype, B)
+        m.set_train_checkpoints(fmt)
+        return m
+    dy = gradient((B, 1, size, size), torch.float32, 1, device)
+    if quick:
+        m = fresh()
+        a, b = (m(x) for x in xs)
+        b.backward(dy)
+        assert torch.equal(flat(m), exact1)
+        m.zero_grad(set_to_none=True)
+        a.backward(dy)
+        assert torch.equal(flat(m), ck0)
+        return
+    exact0, ck1 = lone(xs[0], False), lone(xs[1], True)
+    m = fresh()                                                # one forward, one backward
+    m(xs[0]).backward(dy)
+    assert torch.equal(flat(m), exact0)
+    for order in ((0, 1), (1, 0)):
+        m = fresh()
+        ys = [m(x) for x in xs]
+        got = []
+        for k in order:
+            m.zero_grad(set_to_none=True)
+            ys[k].backward(dy, retain_graph=True)
+            got.append(flat(m))
+        want = [ck0, exact1] if order == (0, 1) else [exact1, ck0]
+        if order == (0, 1):                                    # the newer forward gave way to the older one's backward
+            want = [ck0, ck1]
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+        m.zero_grad(set_to_none=True)
+        ys[0].backward(dy)                                     # a checkpoint may be used again
+        assert torch.equal(flat(m), ck0)
+    m = fresh()                                                # one loss over both: autograd's own order, gradients added
+    a, b = (m(x) for x in xs)
+    torch.autograd.backward([a, b], [dy, dy])
+    assert torch.equal(flat(m), exact1 + ck0) or torch.equal(flat(m), ck0 + ck1)
+    m = fresh()                                                # a forward whose graph is dropped saves nothing
+    a = m(xs[0])
+    del a
+    b = m(xs[1])
+    assert m.engine_for(xs[1], train=True).waiting().checkpoint is None
+    b.backward(dy)
+    assert torch.equal(flat(m), exact1)
