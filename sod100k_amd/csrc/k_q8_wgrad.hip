@@ -7,12 +7,13 @@
 // v_mfma_f32_32x32x16_bf16 as it is.  A float dY is cut by truncation into three bfloat16 numbers of 8 bits each (exact), whose
 // products with X go into the same accumulators: three matrix instructions, nothing lost but the accumulation's own rounding.
 //
-// Block = TM x TN of dW over a slab of the tokens, four waves of (TM / 2) x (TN / 2).  64 tokens are staged at a time into
-// two LDS buffers as [row][64 tokens] bfloat16, a row being an output (dY) or an input channel (X): the operand order of the matrix
-// instruction, 16 bytes = 8 tokens of a channel.  Planar maps hold 8 consecutive pixels of a channel together already; of token rows
-// a thread loads 8 tokens x 4 channels and transposes in registers.  The 16-byte piece c of row r lies at c ^ f(r), f(r) =
-// (r ^ r >> 3) & 7: eight consecutive rows (operand reads) and eight rows four apart (the transposed writes) both fall on
-// eight different pieces.  The global loads of step s + 1 are in flight while step s is multiplied.
+// Block = TM x TN of dW over a slab of the tokens.  64 tokens are staged at a time into two LDS buffers.
+// Planar maps hold eight consecutive pixels of a channel together, an operand of the matrix instruction: LDS rows are channels, [row][64
+// tokens], operands are 128-bit reads.  The 16-byte piece c of row r lies at c ^ f(r), f(r) = (r ^ r >> 3) & 7, so that eight consecutive
+// rows fall on eight different pieces.
+// Token rows hold the channels of a token together: LDS rows are tokens, [64 tokens][row], as they come, and the operands -- eight
+// tokens of a channel -- are formed by the transposing LDS read, four tokens of 16 channels per 16 lanes.  Its four rows' 32 bytes
+// lie in different banks: the 16-byte pieces of token t are exchanged by an xor with 2 (t & 7).
 //
 // Few tiles and many tokens are the usual case (the channels of a map against its pixels), so the tokens are cut into slabs whose
 // partial tiles a second kernel adds in order.
@@ -29,6 +30,11 @@ int64_t csn_q8_wgrad_partial_floats(int, int, int64_t, int64_t, int64_t, int64_t
 #define WG_ROWB 128     // bytes of a staged row
 
 __device__ __forceinline__ unsigned wg_piece(int row, int c) { return (unsigned)(row * WG_ROWB + ((c ^ ((row ^ (row >> 3)) & 7)) << 4)); }
+template <int C>   // token rows of C channels
+__device__ __forceinline__ unsigned wg_token(int t, int piece) {
+  constexpr int M = C >= 128 ? 7 : 3;
+  return (unsigned)(t * (2 * C) + ((piece ^ ((t & M) << 1)) << 4));
+}
 __device__ __forceinline__ csn_u4 wg_u4(unsigned a, unsigned b, unsigned c, unsigned d) {
   csn_u4 r;
   r.x = a; r.y = b; r.z = c; r.w = d;
@@ -93,33 +99,6 @@ template <> struct WgY<float> {
     }
   }
 };
-// four channels of one token of dY
-template <typename AT> struct WgY4;
-template <> struct WgY4<csn_bf16> {
-  uint2 u;
-  __device__ __forceinline__ void zero() { u = make_uint2(0, 0); }
-  __device__ __forceinline__ void load(const csn_bf16* p) { u = *reinterpret_cast<const uint2*>(p); }
-  __device__ __forceinline__ void load_some(const csn_bf16* p, int n) {
-    unsigned short h[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) h[j] = j < n ? p[j].u : (unsigned short)0;
-    u = make_uint2(h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16);
-  }
-  __device__ __forceinline__ float get(int j) const {
-    const unsigned w = j < 2 ? u.x : u.y;
-    return csn_bits_f((j & 1) ? w & 0xffff0000u : w << 16);
-  }
-};
-template <> struct WgY4<float> {
-  float4 a;
-  __device__ __forceinline__ void zero() { a = make_float4(0.f, 0.f, 0.f, 0.f); }
-  __device__ __forceinline__ void load(const float* p) { a = *reinterpret_cast<const float4*>(p); }
-  __device__ __forceinline__ void load_some(const float* p, int n) {
-    a = make_float4(n > 0 ? p[0] : 0.f, n > 1 ? p[1] : 0.f, n > 2 ? p[2] : 0.f, n > 3 ? p[3] : 0.f);
-  }
-  __device__ __forceinline__ float get(int j) const { return j == 0 ? a.x : j == 1 ? a.y : j == 2 ? a.z : a.w; }
-};
-
 // n = 0 .. 4 codes from an address of any alignment
 __device__ __forceinline__ unsigned wg_codes(const uint8_t* p, int n) {
   unsigned w = 0;
@@ -128,24 +107,25 @@ __device__ __forceinline__ unsigned wg_codes(const uint8_t* p, int n) {
   return w;
 }
 
-// what a thread holds of the step in flight
-template <typename AT, bool ROWS, int TM, int TN> struct WgRegs;
-template <typename AT, int TM, int TN> struct WgRegs<AT, false, TM, TN> {
-  WgY<AT> y[TM / 32];
-  uint2 x[TN / 32];
-  unsigned s[TN / 32];
+// waves of a block and their grid over its tile: 64 x 64 .. 128 x 128 on four waves (2 x 2), 256 x 256 on eight (2 x 4)
+template <int TM, int TN> struct WgShape {
+  static constexpr int T = TM == 256 ? 512 : 256, WM = 2, WN = T / 64 / WM;
+  static constexpr int MI = TM / WM / 32, NJ = TN / WN / 32;      // 32 x 32 tiles of a wave
 };
-template <typename AT, int TM, int TN> struct WgRegs<AT, true, TM, TN> {
-  WgY4<AT> y[8];
-  unsigned x[8], s[8];
+// what a thread holds of a step in flight: pieces of eight elements of dY and of X
+template <typename AT, int NY, int NX> struct WgRegs {
+  WgY<AT> y[NY];
+  uint2 x[NX];
+  unsigned s[NX];
 };
 
 template <typename AT, int FMT, bool ROWS, int TM, int TN>
-__global__ __launch_bounds__(CSN_BLOCK) void q8_wgrad_kernel(Q8WgradArgs a) {
+__global__ __launch_bounds__((WgShape<TM, TN>::T)) void q8_wgrad_kernel(Q8WgradArgs a) {
   CSN_DYN_SMEM(unsigned char, sm);
-  constexpr int PARTS = sizeof(AT) == 4 ? 3 : 1;
-  constexpr unsigned YB = TM * WG_ROWB, BUF = PARTS * YB + TN * WG_ROWB;
-  constexpr int MI = TM / 64, NJ = TN / 64;
+  typedef WgShape<TM, TN> S;
+  constexpr int PARTS = sizeof(AT) == 4 ? 3 : 1, T = S::T, MI = S::MI, NJ = S::NJ;
+  constexpr unsigned YB = TM * WG_ROWB, BUF = PARTS * YB + TN * WG_ROWB;   // (64 tokens x TM bfloat16 either way)
+  constexpr int NY = TM * 8 / T, NX = TN * 8 / T;                          // pieces per thread and step
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   // (slab, tile) items in order over the XCDs (block b runs on XCD b % 8): the tiles of a slab read the same tokens, through one L2
   const int ntile = a.mtiles * a.ntiles, total = ntile * a.slabs, per = (total + 7) >> 3;
@@ -154,22 +134,28 @@ __global__ __launch_bounds__(CSN_BLOCK) void q8_wgrad_kernel(Q8WgradArgs a) {
   const int slab = item / ntile, tile = item - slab * ntile;
   const int mt = tile / a.ntiles, nt = tile - mt * a.ntiles;
   const int o0 = mt * TM, i0 = nt * TN;
-  const int s0 = slab * a.steps_per_slab, s1 = min(s0 + a.steps_per_slab, a.steps);
+  const int s0 = slab * a.steps_per_slab, s1 = s0 + a.steps_per_slab;
   const bool bias = a.dbias != nullptr && nt == 0;
 
-  float bsum[4] = {0.f, 0.f, 0.f, 0.f};
-  WgRegs<AT, ROWS, TM, TN> rg;
+  float bsum[ROWS ? 8 : NY];
+#pragma unroll
+  for (int j = 0; j < (ROWS ? 8 : NY); ++j) bsum[j] = 0.f;
+  WgRegs<AT, NY, NX> r0, r1;
+  const bool whole = ROWS && a.vec_y && a.vec_x && o0 + TM <= a.cout && i0 + TN <= a.cin;
+  const int64_t ylane = ROWS ? (int64_t)(tid / (TM / 8)) * a.dy_so + o0 + 8 * (tid % (TM / 8)) : 0;
+  const int64_t xlane = ROWS ? (int64_t)(tid / (TN / 8)) * a.cin + i0 + 8 * (tid % (TN / 8)) : 0;
+  const int64_t elane = ROWS ? (int64_t)(tid / (TN / 8)) * a.nblk + ((i0 + 8 * (tid % (TN / 8))) >> 5) : 0;
 
-  auto load = [&](int step) {
-    if constexpr (!ROWS) {
+  auto load = [&](WgRegs<AT, NY, NX>& rg, int step) {
+    if constexpr (!ROWS) {   // piece j: channel (tid >> 3) + j T / 8, eight pixels number tid & 7 of the step
       const unsigned g = (unsigned)step * 8u + (unsigned)(tid & 7);
       const unsigned o = g / (unsigned)a.chunks, c = g - o * (unsigned)a.chunks;
       const int64_t p = (int64_t)c * 8;
       const int n = (int64_t)o < a.outer ? (int)min((int64_t)8, a.inner - p) : 0;
       const AT* py = reinterpret_cast<const AT*>(a.dy) + (int64_t)o * a.dy_so + p;
 #pragma unroll
-      for (int j = 0; j < TM / 32; ++j) {
-        const int r = o0 + (tid >> 3) + 32 * j;
+      for (int j = 0; j < NY; ++j) {
+        const int r = o0 + (tid >> 3) + T / 8 * j;
         rg.y[j].zero();
         if (r < a.cout && n > 0) {
           if (a.vec_y) rg.y[j].load(py + (int64_t)r * a.dy_sc);
@@ -177,8 +163,8 @@ __global__ __launch_bounds__(CSN_BLOCK) void q8_wgrad_kernel(Q8WgradArgs a) {
         }
       }
 #pragma unroll
-      for (int j = 0; j < TN / 32; ++j) {
-        const int r = i0 + (tid >> 3) + 32 * j;
+      for (int j = 0; j < NX; ++j) {
+        const int r = i0 + (tid >> 3) + T / 8 * j;
         rg.x[j] = make_uint2(0, 0);
         rg.s[j] = 127;
         if (r < a.cin && n > 0) {
@@ -189,33 +175,48 @@ __global__ __launch_bounds__(CSN_BLOCK) void q8_wgrad_kernel(Q8WgradArgs a) {
           rg.s[j] = a.exps[row * a.nblk + (p >> 5)];
         }
       }
-    } else {
-      constexpr int GY = TM / 4, GX = TN / 4;
-      {
-        const int c = o0 + 4 * (tid & (GY - 1)), k = tid / GY;
-        const int n = k < 8 ? (int)min((int64_t)4, a.cout - c) : 0;
+    } else {                 // piece j: token tid / (TM / 8) + j T / (TM / 8) of the step, eight channels number tid % (TM / 8)
+      const int64_t t0 = (int64_t)step * WG_STEP;
+      if (whole && t0 + WG_STEP <= a.outer) {   // (uniform: no bounds inside)
+        constexpr int GY = TM / 8, GX = TN / 8;
+        const AT* py = reinterpret_cast<const AT*>(a.dy) + t0 * a.dy_so;
+        const uint8_t* px = a.codes + t0 * a.cin;
+        const uint8_t* pe = a.exps + t0 * a.nblk;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int64_t t = (int64_t)step * WG_STEP + 8 * k + j;
+        for (int j = 0; j < NY; ++j) rg.y[j].load(py + (int64_t)(T / GY * j) * a.dy_so + ylane);
+#pragma unroll
+        for (int j = 0; j < NX; ++j) {
+          rg.x[j] = *reinterpret_cast<const uint2*>(px + (int64_t)(T / GX * j) * a.cin + xlane);
+          rg.s[j] = *(pe + (int64_t)(T / GX * j) * a.nblk + elane);
+        }
+        return;
+      }
+      {
+        constexpr int G = TM / 8;
+        const int c = o0 + 8 * (tid % G), n = (int)min((int64_t)8, a.cout - c);
+#pragma unroll
+        for (int j = 0; j < NY; ++j) {
+          const int64_t t = t0 + tid / G + T / G * j;
           rg.y[j].zero();
           if (n > 0 && t < a.outer) {
             const AT* py = reinterpret_cast<const AT*>(a.dy) + t * a.dy_so + c;
-            if (a.vec_y && n == 4) rg.y[j].load(py);
+            if (a.vec_y && n == 8) rg.y[j].load(py);
             else rg.y[j].load_some(py, n);
           }
         }
       }
       {
-        const int c = i0 + 4 * (tid & (GX - 1)), k = tid / GX;
-        const int n = k < 8 ? (int)min((int64_t)4, a.cin - c) : 0;
+        constexpr int G = TN / 8;
+        const int c = i0 + 8 * (tid % G), n = (int)min((int64_t)8, a.cin - c);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int64_t t = (int64_t)step * WG_STEP + 8 * k + j;
-          rg.x[j] = 0;
+        for (int j = 0; j < NX; ++j) {
+          const int64_t t = t0 + tid / G + T / G * j;
+          rg.x[j] = make_uint2(0, 0);
           rg.s[j] = 127;
           if (n > 0 && t < a.outer) {
             const uint8_t* px = a.codes + t * a.cin + c;
-            rg.x[j] = a.vec_x && n == 4 ? *reinterpret_cast<const unsigned*>(px) : wg_codes(px, n);
+            if (a.vec_x && n == 8) rg.x[j] = *reinterpret_cast<const uint2*>(px);
+            else rg.x[j] = make_uint2(wg_codes(px, n), wg_codes(px + 4, n - 4));
             rg.s[j] = a.exps[t * a.nblk + (c >> 5)];
           }
         }
@@ -223,60 +224,34 @@ __global__ __launch_bounds__(CSN_BLOCK) void q8_wgrad_kernel(Q8WgradArgs a) {
     }
   };
 
-  auto store = [&](unsigned char* buf) {
+  auto store = [&](const WgRegs<AT, NY, NX>& rg, unsigned char* buf) {
     unsigned char* bx = buf + PARTS * YB;
-    if constexpr (!ROWS) {
 #pragma unroll
-      for (int j = 0; j < TM / 32; ++j) {
-        rg.y[j].put(buf, wg_piece((tid >> 3) + 32 * j, tid & 7), YB);
-        if (bias) {
-          float f[8];
-          rg.y[j].get(f);
-          bsum[j] += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < TN / 32; ++j) {
-        const float sc = q8_scale(rg.s[j]);
-        const unsigned w[2] = {rg.x[j].x, rg.x[j].y};
+    for (int j = 0; j < NY; ++j) {
+      unsigned at;
+      if constexpr (!ROWS) at = wg_piece((tid >> 3) + T / 8 * j, tid & 7);
+      else at = wg_token<TM>(tid / (TM / 8) + T / (TM / 8) * j, tid % (TM / 8));
+      rg.y[j].put(buf, at, YB);
+      if (bias) {
         float f[8];
-        q8_decode_vec<FMT, 8>(w, sc, f);
-        *reinterpret_cast<csn_u4*>(bx + wg_piece((tid >> 3) + 32 * j, tid & 7)) =
-            wg_u4(wg_hi2(f[0], f[1]), wg_hi2(f[2], f[3]), wg_hi2(f[4], f[5]), wg_hi2(f[6], f[7]));
-      }
-    } else {
-      constexpr int GY = TM / 4, GX = TN / 4;
-      if (tid / GY < 8) {
-        const int c = 4 * (tid & (GY - 1)), k = tid / GY;
+        rg.y[j].get(f);
+        if constexpr (!ROWS) {
+          bsum[j] += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+        } else {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float f[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] = rg.y[j].get(q);
-          if (bias) bsum[q] += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
-#pragma unroll
-          for (int part = 0; part < PARTS; ++part) {
-            float h[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) h[j] = PARTS == 1 ? f[j] : wg_cut(f[j]);
-            *reinterpret_cast<csn_u4*>(buf + part * YB + wg_piece(c + q, k)) =
-                wg_u4(wg_hi2(h[0], h[1]), wg_hi2(h[2], h[3]), wg_hi2(h[4], h[5]), wg_hi2(h[6], h[7]));
-          }
+          for (int q = 0; q < 8; ++q) bsum[q] += f[q];
         }
       }
-      if (tid / GX < 8) {
-        const int c = 4 * (tid & (GX - 1)), k = tid / GX;
-        float f[8][4];
+    }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const unsigned w[1] = {rg.x[j]};
-          q8_decode_vec<FMT, 4>(w, q8_scale(rg.s[j]), f[j]);
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<csn_u4*>(bx + wg_piece(c + q, k)) =
-              wg_u4(wg_hi2(f[0][q], f[1][q]), wg_hi2(f[2][q], f[3][q]), wg_hi2(f[4][q], f[5][q]), wg_hi2(f[6][q], f[7][q]));
-      }
+    for (int j = 0; j < NX; ++j) {
+      unsigned at;
+      if constexpr (!ROWS) at = wg_piece((tid >> 3) + T / 8 * j, tid & 7);
+      else at = wg_token<TN>(tid / (TN / 8) + T / (TN / 8) * j, tid % (TN / 8));
+      const unsigned w[2] = {rg.x[j].x, rg.x[j].y};
+      float f[8];
+      q8_decode_vec<FMT, 8>(w, q8_scale(rg.s[j]), f);
+      *reinterpret_cast<csn_u4*>(bx + at) = wg_u4(wg_hi2(f[0], f[1]), wg_hi2(f[2], f[3]), wg_hi2(f[4], f[5]), wg_hi2(f[6], f[7]));
     }
   };
 
@@ -288,33 +263,75 @@ __global__ __launch_bounds__(CSN_BLOCK) void q8_wgrad_kernel(Q8WgradArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  const int wr = (wave >> 1) * (TM / 2), wc = (wave & 1) * (TN / 2);
-  int cur = 0;
-  if (s0 < s1) {
-    load(s0);
-    store(sm);
+  const int wr = (wave / S::WN) * (TM / S::WM), wc = (wave % S::WN) * (TN / S::WN);
+  // Operand of 32 channels, tokens 16 kk + 8 (lane >> 5) .. + 7.  Of token rows: two transposing reads of four tokens each, whose addresses
+  // in the first 16 tokens are kept (the pieces' exchange depends on the token modulo 8 alone).
+  unsigned ya[ROWS ? MI : 1][2], xa[ROWS ? NJ : 1][2];
+  if constexpr (ROWS) {
+    const int t = 8 * (lane >> 5) + ((lane & 15) >> 2), ch = (lane & 16) + 4 * (lane & 3);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < MI; ++i) ya[i][h] = wg_token<TM>(t + 4 * h, (wr + 32 * i + ch) >> 3) + 2u * (ch & 4);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) xa[j][h] = PARTS * YB + wg_token<TN>(t + 4 * h, (wc + 32 * j + ch) >> 3) + 2u * (ch & 4);
+    }
   }
-  for (int s = s0; s < s1; ++s) {
-    if (s + 1 < s1) load(s + 1);
-    __syncthreads();
-    const unsigned char* buf = sm + cur * BUF;
+  auto read8 = [&](const unsigned char* p, const unsigned char* q) {
+    const uint2 lo = csn_lds_read_tr16(p), hi = csn_lds_read_tr16(q);
+    return wg_u4(lo.x, lo.y, hi.x, hi.y);
+  };
+  auto multiply = [&](const unsigned char* buf) {
 #pragma unroll
     for (int kk = 0; kk < WG_STEP / 16; ++kk) {
-      const int c = 2 * kk + (lane >> 5);
       csn_u4 b[NJ];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) b[j] = *reinterpret_cast<const csn_u4*>(buf + PARTS * YB + wg_piece(wc + 32 * j + (lane & 31), c));
+      for (int j = 0; j < NJ; ++j) {
+        if constexpr (ROWS) b[j] = read8(buf + xa[j][0] + 32 * TN * kk, buf + xa[j][1] + 32 * TN * kk);
+        else b[j] = *reinterpret_cast<const csn_u4*>(buf + PARTS * YB + wg_piece(wc + 32 * j + (lane & 31), 2 * kk + (lane >> 5)));
+      }
 #pragma unroll
       for (int part = 0; part < PARTS; ++part)
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
-          const csn_u4 y = *reinterpret_cast<const csn_u4*>(buf + part * YB + wg_piece(wr + 32 * i + (lane & 31), c));
+          csn_u4 y;
+          if constexpr (ROWS) y = read8(buf + part * YB + ya[i][0] + 32 * TM * kk, buf + part * YB + ya[i][1] + 32 * TM * kk);
+          else y = *reinterpret_cast<const csn_u4*>(buf + part * YB + wg_piece(wr + 32 * i + (lane & 31), 2 * kk + (lane >> 5)));
 #pragma unroll
           for (int j = 0; j < NJ; ++j) acc[i][j] = csn_mfma_32x32x16_bf16(y, b[j], acc[i][j]);
         }
+      if constexpr (TM == 256) CSN_SCHED_FENCE();   // (operands of one kk at a time: the accumulators take half of the registers)
     }
-    cur ^= 1;
-    if (s + 1 < s1) store(sm + cur * BUF);
+  };
+  // The slab's steps in pairs (steps_per_slab is even, tokens behind the last read as zeros).  Two register sets: the registers of a step
+  // are free again once it lies in its buffer, and hold the step two further on while the buffers are multiplied.  The large tile's
+  // accumulators leave room for one set, one step ahead.
+  constexpr bool TWO = TM < 256;
+  load(r0, s0);
+  if constexpr (TWO) load(r1, s0 + 1);
+  store(r0, sm);
+#pragma unroll 1
+  for (int s = s0; s < s1; s += 2) {
+    const bool more = s + 2 < s1;
+    if constexpr (TWO) {
+      if (more) load(r0, s + 2);
+      __syncthreads();
+      multiply(sm);
+      store(r1, sm + BUF);
+      if (more) load(r1, s + 3);
+      __syncthreads();
+      multiply(sm + BUF);
+      if (more) store(r0, sm);
+    } else {
+      load(r0, s + 1);
+      __syncthreads();
+      multiply(sm);
+      store(r0, sm + BUF);
+      if (more) load(r0, s + 2);
+      __syncthreads();
+      multiply(sm + BUF);
+      if (more) store(r0, sm);
+    }
   }
 
   float* out = a.slabs > 1 ? a.partial + (int64_t)slab * a.cout * (a.cin + 1) : a.dweight;
@@ -330,23 +347,21 @@ __global__ __launch_bounds__(CSN_BLOCK) void q8_wgrad_kernel(Q8WgradArgs a) {
           if (c < a.cin) out[o * a.cin + c] = acc[i][j][r];
         }
     }
-  if (bias) {   // the block's sums of dY: eight threads hold a row's
+  if (bias) {   // the block's sums of dY: K threads hold a channel's
+    constexpr int K = ROWS ? T / (TM / 8) : 8;
     __syncthreads();
-    float* sb = reinterpret_cast<float*>(sm);   // [TM][8]
+    float* sb = reinterpret_cast<float*>(sm);   // [TM][K]
     if constexpr (!ROWS) {
 #pragma unroll
-      for (int j = 0; j < TM / 32; ++j) sb[((tid >> 3) + 32 * j) * 8 + (tid & 7)] = bsum[j];
+      for (int j = 0; j < NY; ++j) sb[((tid >> 3) + T / 8 * j) * K + (tid & 7)] = bsum[j];
     } else {
-      constexpr int GY = TM / 4;
-      if (tid / GY < 8)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) sb[(4 * (tid & (GY - 1)) + q) * 8 + tid / GY] = bsum[q];
+      for (int q = 0; q < 8; ++q) sb[(8 * (tid % (TM / 8)) + q) * K + tid / (TM / 8)] = bsum[q];
     }
     __syncthreads();
     if (tid < TM && o0 + tid < a.cout) {
       float v = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v += sb[tid * 8 + j];
+      for (int j = 0; j < K; ++j) v += sb[tid * K + j];
       (a.slabs > 1 ? out + a.cout * a.cin : a.dbias)[o0 + tid] = v;   // (behind the slab's dW)
     }
   }
@@ -354,29 +369,32 @@ __global__ __launch_bounds__(CSN_BLOCK) void q8_wgrad_kernel(Q8WgradArgs a) {
 
 struct WgPlan { int tm, tn, mtiles, ntiles, steps, steps_per_slab, slabs, chunks; };
 
-// Tiles of 128 where the channels fill more than 64.  About 512 blocks (two per CU), but at least four steps of 64 tokens each: a
-// slab costs a partial tile written and read again.
-static bool wg_plan(int rows, int64_t outer, int64_t inner, int64_t cin, int64_t cout, WgPlan& p) {
-  p.tm = cout > 64 ? 128 : 64;
-  p.tn = cin > 64 ? 128 : 64;
-  const int64_t mt = (cout + p.tm - 1) / p.tm, nt = (cin + p.tn - 1) / p.tn;
+// Tiles of 128 where the channels fill more than 64; of 256 x 256, whose operands are read from LDS half as often, where there are enough of
+// them times steps for every CU (bfloat16 dY: the three parts of a float one do not fit).  About two blocks per CU -- one of the large tile --
+// but at least four steps of 64 tokens each: a slab costs a partial tile written and read again.
+static bool wg_plan(int rows, int a16, int64_t outer, int64_t inner, int64_t cin, int64_t cout, WgPlan& p) {
   const int64_t chunks = rows ? 1 : (inner + 7) / 8;
   const int64_t all = rows ? (outer + 7) / 8 : outer * chunks, steps = (all + 7) / 8;
+  p.tm = cout > 64 ? 128 : 64;
+  p.tn = cin > 64 ? 128 : 64;
+  const bool big = rows && a16 && cout > 128 && cin > 128 && ((cout + 255) / 256) * ((cin + 255) / 256) * steps >= 256 * 8;
+  if (big) p.tm = p.tn = 256;
+  const int64_t mt = (cout + p.tm - 1) / p.tm, nt = (cin + p.tn - 1) / p.tn;
   if (mt * nt > (1 << 20) || all > 0x7ffffff0LL || chunks > 0x7ffffff0LL) return false;
-  int64_t slabs = (512 + mt * nt - 1) / (mt * nt);
+  int64_t slabs = ((big ? 256 : 512) + mt * nt - 1) / (mt * nt);
   slabs = std::min(slabs, (steps + 3) / 4);
   if (slabs < 1) slabs = 1;
   p.mtiles = (int)mt; p.ntiles = (int)nt; p.steps = (int)steps; p.chunks = (int)(chunks < 1 ? 1 : chunks);
-  p.steps_per_slab = (int)((steps + slabs - 1) / slabs);
-  if (p.steps_per_slab < 1) p.steps_per_slab = 1;
+  p.steps_per_slab = ((int)((steps + slabs - 1) / slabs) + 1) & ~1;
+  if (p.steps_per_slab < 2) p.steps_per_slab = 2;
   p.slabs = (int)((steps + p.steps_per_slab - 1) / p.steps_per_slab);
   if (p.slabs < 1) p.slabs = 1;
   return true;
 }
 
-int64_t csn_q8_wgrad_partial_floats(int rows, int, int64_t outer, int64_t inner, int64_t cin, int64_t cout) {
+int64_t csn_q8_wgrad_partial_floats(int rows, int a16, int64_t outer, int64_t inner, int64_t cin, int64_t cout) {
   WgPlan p;
-  if (!wg_plan(rows, outer, inner, cin, cout, p) || p.slabs <= 1) return 0;
+  if (!wg_plan(rows, a16, outer, inner, cin, cout, p) || p.slabs <= 1) return 0;
   return (int64_t)p.slabs * (cout * cin + cout);
 }
 
@@ -392,7 +410,7 @@ static int q8_wgrad_run(const Q8WgradArgs& a, void* stream) {
   if (st != 0) return st;
 #endif
   const int total = a.mtiles * a.ntiles * a.slabs;
-  CSN_LAUNCH((q8_wgrad_kernel<AT, FMT, ROWS, TM, TN>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(CSN_BLOCK), smem, stream, a);
+  CSN_LAUNCH((q8_wgrad_kernel<AT, FMT, ROWS, TM, TN>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(WgShape<TM, TN>::T), smem, stream, a);
   if (a.slabs > 1) {
     const int e = (int)hipGetLastError();
     if (e != 0) return e;
@@ -405,6 +423,8 @@ static int q8_wgrad_run(const Q8WgradArgs& a, void* stream) {
 
 template <typename AT, int FMT, bool ROWS>
 static int q8_wgrad_tile(const Q8WgradArgs& a, const WgPlan& p, void* stream) {
+  if constexpr (ROWS && sizeof(AT) == 2)
+    if (p.tm == 256) return q8_wgrad_run<AT, FMT, ROWS, 256, 256>(a, stream);
   if (p.tm == 128) return p.tn == 128 ? q8_wgrad_run<AT, FMT, ROWS, 128, 128>(a, stream) : q8_wgrad_run<AT, FMT, ROWS, 128, 64>(a, stream);
   return p.tn == 128 ? q8_wgrad_run<AT, FMT, ROWS, 64, 128>(a, stream) : q8_wgrad_run<AT, FMT, ROWS, 64, 64>(a, stream);
 }
@@ -412,12 +432,12 @@ static int q8_wgrad_tile(const Q8WgradArgs& a, const WgPlan& p, void* stream) {
 int csn_launch_q8_wgrad(const Q8WgradArgs& a0, int rows, int a16, int fmt, void* stream) {
   Q8WgradArgs a = a0;
   WgPlan p;
-  if (!wg_plan(rows, a.outer, a.inner, a.cin, a.cout, p)) return -1;
+  if (!wg_plan(rows, a16, a.outer, a.inner, a.cin, a.cout, p)) return -1;
   a.mtiles = p.mtiles; a.ntiles = p.ntiles; a.steps = p.steps; a.steps_per_slab = p.steps_per_slab; a.slabs = p.slabs; a.chunks = p.chunks;
-  const uintptr_t es = a16 ? 2 : 4, py = (uintptr_t)a.dy, px = (uintptr_t)a.codes;
-  if (rows) {   // 4 channels of a token at once
-    a.vec_y = py % (4 * es) == 0 && a.dy_so % 4 == 0;
-    a.vec_x = px % 4 == 0 && a.cin % 4 == 0;
+  const uintptr_t py = (uintptr_t)a.dy, px = (uintptr_t)a.codes;
+  if (rows) {   // 8 channels of a token at once
+    a.vec_y = py % 16 == 0 && a.dy_so % 8 == 0;
+    a.vec_x = px % 8 == 0 && a.cin % 8 == 0;
   } else {      // 8 pixels of a channel at once, no plane ending inside them
     a.vec_y = a.inner % 8 == 0 && py % 16 == 0 && a.dy_so % 8 == 0 && a.dy_sc % 8 == 0;
     a.vec_x = a.inner % 8 == 0 && px % 8 == 0;

@@ -75,7 +75,7 @@ def test_gpu_norm(lib, shape, dim, dtype):
 @pytest.mark.parametrize("dtype", K.DTYPES)
 def test_gpu_product_gradient(lib, dtype, fmt):
     for i, (dims, cin, cout, dim) in enumerate(K.PRODUCT_SHAPES + [((513,), 300, 280, -1), ((2, 31, 33), 129, 257, 1), ((3, 24, 24), 256, 128, 1),
-                                                                   ((1030,), 128, 512, -1)]):
+                                                                   ((1030,), 128, 512, -1), ((2051,), 500, 1200, -1), ((70000,), 264, 257, -1)]):
         x, dy = K.product_tensors(dims, cin, cout, dim, dtype, i, DEV)
         K.check_product(lib, dy, x, fmt, dim)
 
