@@ -20,6 +20,7 @@
 #include "q8_core.h"
 #include "slab_sum.h"
 #include "train_ops.h"
+#include "vec_io.h"
 
 #ifdef CSN_EMU_SEQ
 int csn_launch_q8_wgrad(const Q8WgradArgs&, int, int, int, void*) { return -1; }   // (matrix instructions: lane-exact mode only)
@@ -55,37 +56,37 @@ __device__ __forceinline__ float wg_cut(float& x) {
   return h;
 }
 
-// eight tokens of one row of dY as they were loaded
+// eight consecutive elements of dY as they were loaded
 template <typename AT> struct WgY;
 template <> struct WgY<csn_bf16> {
-  uint4 u;
-  __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ void load(const csn_bf16* p) { u = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void load_some(const csn_bf16* p, int n) {
-    unsigned short h[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) h[j] = j < n ? p[j].u : (unsigned short)0;
-    u = make_uint4(h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16, h[4] | (unsigned)h[5] << 16, h[6] | (unsigned)h[7] << 16);
+  VecIo<csn_bf16> v;
+  __device__ __forceinline__ void zero() { v.zero(); }
+  __device__ __forceinline__ void load(const csn_bf16* p) { v.load(p); }
+  __device__ __forceinline__ void load_each(const csn_bf16* p, int n) { v.load_each(p, n); }
+  __device__ __forceinline__ void shift(int s) { v.shift(s); }
+  __device__ __forceinline__ void get(float (&f)[8]) const { v.get(f); }
+  __device__ __forceinline__ void put(unsigned char* lds, unsigned at, unsigned) const {
+    *reinterpret_cast<csn_u4*>(lds + at) = wg_u4(v.w[0], v.w[1], v.w[2], v.w[3]);
   }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
-    const unsigned w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) { f[2 * j] = csn_bits_f(w[j] << 16); f[2 * j + 1] = csn_bits_f(w[j] & 0xffff0000u); }
-  }
-  __device__ __forceinline__ void put(unsigned char* lds, unsigned at, unsigned) const { *reinterpret_cast<csn_u4*>(lds + at) = wg_u4(u.x, u.y, u.z, u.w); }
 };
 template <> struct WgY<float> {
-  float4 a, b;
-  __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
-  __device__ __forceinline__ void load(const float* p) { a = *reinterpret_cast<const float4*>(p); b = *reinterpret_cast<const float4*>(p + 4); }
-  __device__ __forceinline__ void load_some(const float* p, int n) {
-    float f[8];
+  VecIo<float> a, b;
+  __device__ __forceinline__ void zero() { a.zero(); b.zero(); }
+  __device__ __forceinline__ void load(const float* p) { a.load(p); b.load(p + 4); }
+  __device__ __forceinline__ void load_each(const float* p, int n) { a.load_each(p, n); b.load_each(p + 4, n - 4); }
+  __device__ __forceinline__ void shift(int s) {   // drop the first s < 8 elements
+    if (s & 4) { a = b; b.zero(); }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = j < n ? p[j] : 0.f;
-    a = make_float4(f[0], f[1], f[2], f[3]); b = make_float4(f[4], f[5], f[6], f[7]);
+    for (int k = 2; k; k >>= 1)
+      if (s & k) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a.w[j] = j + k < 4 ? a.w[(j + k) & 3] : b.w[(j + k) & 3];
+        b.shift(k);
+      }
   }
   __device__ __forceinline__ void get(float (&f)[8]) const {
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { f[j] = csn_bits_f(a.w[j]); f[4 + j] = csn_bits_f(b.w[j]); }
   }
   __device__ __forceinline__ void put(unsigned char* lds, unsigned at, unsigned part) const {
     float f[8];
@@ -99,27 +100,24 @@ template <> struct WgY<float> {
     }
   }
 };
-// n = 0 .. 4 codes from an address of any alignment
-__device__ __forceinline__ unsigned wg_codes(const uint8_t* p, int n) {
-  unsigned w = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) w |= j < n ? (unsigned)p[j] << (8 * j) : 0u;
-  return w;
-}
 
 // waves of a block and their grid over its tile: 64 x 64 .. 128 x 128 on four waves (2 x 2), 256 x 256 on eight (2 x 4)
 template <int TM, int TN> struct WgShape {
   static constexpr int T = TM == 256 ? 512 : 256, WM = 2, WN = T / 64 / WM;
   static constexpr int MI = TM / WM / 32, NJ = TN / WN / 32;      // 32 x 32 tiles of a wave
 };
-// what a thread holds of a step in flight: pieces of eight elements of dY and of X
+// what a thread holds of a step in flight: pieces of eight elements of dY and of X (planar: n pixels of each are the map's)
 template <typename AT, int NY, int NX> struct WgRegs {
   WgY<AT> y[NY];
-  uint2 x[NX];
+  CodeIo<8> x[NX];
   unsigned s[NX];
+  int n;
 };
 
-template <typename AT, int FMT, bool ROWS, int TM, int TN>
+// WIDE: a plane / a token of either tensor has at least eight elements.  A piece that reaches past its end is then loaded stepped back
+// and shifted (vec_io.h); channels past the last one are loaded from inside the tensor -- every entry of dW is a sum of its own and
+// those are not stored -- and only tokens past the last one are cleared.
+template <typename AT, int FMT, bool ROWS, bool WIDE, int TM, int TN>
 __global__ __launch_bounds__((WgShape<TM, TN>::T)) void q8_wgrad_kernel(Q8WgradArgs a) {
   CSN_DYN_SMEM(unsigned char, sm);
   typedef WgShape<TM, TN> S;
@@ -141,91 +139,122 @@ __global__ __launch_bounds__((WgShape<TM, TN>::T)) void q8_wgrad_kernel(Q8WgradA
 #pragma unroll
   for (int j = 0; j < (ROWS ? 8 : NY); ++j) bsum[j] = 0.f;
   WgRegs<AT, NY, NX> r0, r1;
-  const bool whole = ROWS && a.vec_y && a.vec_x && o0 + TM <= a.cout && i0 + TN <= a.cin;
-  const int64_t ylane = ROWS ? (int64_t)(tid / (TM / 8)) * a.dy_so + o0 + 8 * (tid % (TM / 8)) : 0;
-  const int64_t xlane = ROWS ? (int64_t)(tid / (TN / 8)) * a.cin + i0 + 8 * (tid % (TN / 8)) : 0;
-  const int64_t elane = ROWS ? (int64_t)(tid / (TN / 8)) * a.nblk + ((i0 + 8 * (tid % (TN / 8))) >> 5) : 0;
 
   auto load = [&](WgRegs<AT, NY, NX>& rg, int step) {
     if constexpr (!ROWS) {   // piece j: channel (tid >> 3) + j T / 8, eight pixels number tid & 7 of the step
       const unsigned g = (unsigned)step * 8u + (unsigned)(tid & 7);
-      const unsigned o = g / (unsigned)a.chunks, c = g - o * (unsigned)a.chunks;
+      unsigned o = g / (unsigned)a.chunks, c = g - o * (unsigned)a.chunks;
+      const bool in = (int64_t)o < a.outer;
+      if (!in) { o = (unsigned)a.outer - 1; c = 0; }
       const int64_t p = (int64_t)c * 8;
-      const int n = (int64_t)o < a.outer ? (int)min((int64_t)8, a.inner - p) : 0;
+      const int left = (int)min((int64_t)8, a.inner - p), n = in ? left : 0;
+      rg.n = n;
       const AT* py = reinterpret_cast<const AT*>(a.dy) + (int64_t)o * a.dy_so + p;
+      const int64_t row0 = (int64_t)o * a.cin;
+      if constexpr (WIDE) {
+        py -= 8 - left;
 #pragma unroll
-      for (int j = 0; j < NY; ++j) {
-        const int r = o0 + (tid >> 3) + T / 8 * j;
-        rg.y[j].zero();
-        if (r < a.cout && n > 0) {
-          if (a.vec_y) rg.y[j].load(py + (int64_t)r * a.dy_sc);
-          else rg.y[j].load_some(py + (int64_t)r * a.dy_sc, n);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < NX; ++j) {
-        const int r = i0 + (tid >> 3) + T / 8 * j;
-        rg.x[j] = make_uint2(0, 0);
-        rg.s[j] = 127;
-        if (r < a.cin && n > 0) {
-          const int64_t row = (int64_t)o * a.cin + r;
-          const uint8_t* px = a.codes + row * a.inner + p;
-          if (a.vec_x) rg.x[j] = *reinterpret_cast<const uint2*>(px);
-          else rg.x[j] = make_uint2(wg_codes(px, n), wg_codes(px + 4, n - 4));
-          rg.s[j] = a.exps[row * a.nblk + (p >> 5)];
-        }
-      }
-    } else {                 // piece j: token tid / (TM / 8) + j T / (TM / 8) of the step, eight channels number tid % (TM / 8)
-      const int64_t t0 = (int64_t)step * WG_STEP;
-      if (whole && t0 + WG_STEP <= a.outer) {   // (uniform: no bounds inside)
-        constexpr int GY = TM / 8, GX = TN / 8;
-        const AT* py = reinterpret_cast<const AT*>(a.dy) + t0 * a.dy_so;
-        const uint8_t* px = a.codes + t0 * a.cin;
-        const uint8_t* pe = a.exps + t0 * a.nblk;
-#pragma unroll
-        for (int j = 0; j < NY; ++j) rg.y[j].load(py + (int64_t)(T / GY * j) * a.dy_so + ylane);
+        for (int j = 0; j < NY; ++j) rg.y[j].load(py + (int64_t)min((int64_t)(o0 + (tid >> 3) + T / 8 * j), a.cout - 1) * a.dy_sc);
 #pragma unroll
         for (int j = 0; j < NX; ++j) {
-          rg.x[j] = *reinterpret_cast<const uint2*>(px + (int64_t)(T / GX * j) * a.cin + xlane);
-          rg.s[j] = *(pe + (int64_t)(T / GX * j) * a.nblk + elane);
+          const int64_t row = row0 + min((int64_t)(i0 + (tid >> 3) + T / 8 * j), a.cin - 1);
+          rg.x[j].load(a.codes + row * a.inner + p - (8 - left));
+          rg.s[j] = a.exps[row * a.nblk + (p >> 5)];
         }
-        return;
-      }
-      {
-        constexpr int G = TM / 8;
-        const int c = o0 + 8 * (tid % G), n = (int)min((int64_t)8, a.cout - c);
+      } else {
 #pragma unroll
         for (int j = 0; j < NY; ++j) {
-          const int64_t t = t0 + tid / G + T / G * j;
+          const int r = o0 + (tid >> 3) + T / 8 * j;
           rg.y[j].zero();
-          if (n > 0 && t < a.outer) {
-            const AT* py = reinterpret_cast<const AT*>(a.dy) + t * a.dy_so + c;
-            if (a.vec_y && n == 8) rg.y[j].load(py);
-            else rg.y[j].load_some(py, n);
+          if (r < a.cout) rg.y[j].load_each(py + (int64_t)r * a.dy_sc, n);
+        }
+#pragma unroll
+        for (int j = 0; j < NX; ++j) {
+          const int r = i0 + (tid >> 3) + T / 8 * j;
+          rg.x[j].zero();
+          rg.s[j] = 127;
+          if (r < a.cin && n > 0) {
+            code_load<false, 8>(rg.x[j], a.codes + (row0 + r) * a.inner + p, n);
+            rg.s[j] = a.exps[(row0 + r) * a.nblk + (p >> 5)];
           }
         }
       }
-      {
-        constexpr int G = TN / 8;
-        const int c = i0 + 8 * (tid % G), n = (int)min((int64_t)8, a.cin - c);
+    } else {                 // piece j: token tid / (TM / 8) + j T / (TM / 8) of the step, eight channels number tid % (TM / 8)
+      constexpr int GY = TM / 8, GX = TN / 8;
+      const int64_t t0 = (int64_t)step * WG_STEP;
+      const int cy = o0 + 8 * (tid % GY), cx = i0 + 8 * (tid % GX);
+      if constexpr (WIDE) {
+        const int by = min(cy, (int)a.cout - 8), bx = min(cx, (int)a.cin - 8);   // (stepped back; wholly outside: anywhere)
+        const int64_t last = a.outer - 1 - t0;
+#pragma unroll
+        for (int j = 0; j < NY; ++j)
+          rg.y[j].load(reinterpret_cast<const AT*>(a.dy) + (t0 + min((int64_t)(tid / GY + T / GY * j), last)) * a.dy_so + by);
 #pragma unroll
         for (int j = 0; j < NX; ++j) {
-          const int64_t t = t0 + tid / G + T / G * j;
-          rg.x[j] = make_uint2(0, 0);
+          const int64_t t = t0 + min((int64_t)(tid / GX + T / GX * j), last);
+          rg.x[j].load(a.codes + t * a.cin + bx);
+          rg.s[j] = a.exps[t * a.nblk + (min(cx, (int)a.cin - 1) >> 5)];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NY; ++j) {
+          const int64_t t = t0 + tid / GY + T / GY * j;
+          rg.y[j].zero();
+          if (t < a.outer) rg.y[j].load_each(reinterpret_cast<const AT*>(a.dy) + t * a.dy_so + cy, (int)min((int64_t)8, a.cout - cy));
+        }
+#pragma unroll
+        for (int j = 0; j < NX; ++j) {
+          const int64_t t = t0 + tid / GX + T / GX * j;
+          rg.x[j].zero();
           rg.s[j] = 127;
-          if (n > 0 && t < a.outer) {
-            const uint8_t* px = a.codes + t * a.cin + c;
-            if (a.vec_x && n == 8) rg.x[j] = *reinterpret_cast<const uint2*>(px);
-            else rg.x[j] = make_uint2(wg_codes(px, n), wg_codes(px + 4, n - 4));
-            rg.s[j] = a.exps[t * a.nblk + (c >> 5)];
+          if (t < a.outer && cx < a.cin) {
+            code_load<false, 8>(rg.x[j], a.codes + t * a.cin + cx, (int)min((int64_t)8, a.cin - cx));
+            rg.s[j] = a.exps[t * a.nblk + (cx >> 5)];
           }
         }
       }
     }
   };
+  // what the loads brought that is not the tensors': shifted down or cleared
+  auto finish = [&](WgRegs<AT, NY, NX>& rg, int step) {
+    if constexpr (WIDE && !ROWS) {
+      if (rg.n < 8) {
+#pragma unroll
+        for (int j = 0; j < NY; ++j) {
+          if (rg.n > 0) rg.y[j].shift(8 - rg.n);
+          else rg.y[j].zero();
+        }
+#pragma unroll
+        for (int j = 0; j < NX; ++j) {
+          if (rg.n > 0) code_end<true, 8>(rg.x[j], rg.n);
+          else rg.x[j].zero();
+        }
+      }
+    }
+    if constexpr (WIDE && ROWS) {
+      constexpr int GY = TM / 8, GX = TN / 8;
+      const int64_t t0 = (int64_t)step * WG_STEP;
+      const int cy = o0 + 8 * (tid % GY), cx = i0 + 8 * (tid % GX);
+      if (o0 + TM > a.cout && cy < a.cout && cy + 8 > a.cout)
+#pragma unroll
+        for (int j = 0; j < NY; ++j) rg.y[j].shift(cy + 8 - (int)a.cout);
+      if (i0 + TN > a.cin && cx < a.cin && cx + 8 > a.cin)
+#pragma unroll
+        for (int j = 0; j < NX; ++j) code_end<true, 8>(rg.x[j], (int)a.cin - cx);
+      if (t0 + WG_STEP > a.outer) {
+#pragma unroll
+        for (int j = 0; j < NY; ++j)
+          if (t0 + tid / GY + T / GY * j >= a.outer) rg.y[j].zero();
+#pragma unroll
+        for (int j = 0; j < NX; ++j)
+          if (t0 + tid / GX + T / GX * j >= a.outer) rg.x[j].zero();
+      }
+    }
+  };
 
-  auto store = [&](const WgRegs<AT, NY, NX>& rg, unsigned char* buf) {
+  auto store = [&](WgRegs<AT, NY, NX>& rg, int step, unsigned char* buf) {
     unsigned char* bx = buf + PARTS * YB;
+    finish(rg, step);
 #pragma unroll
     for (int j = 0; j < NY; ++j) {
       unsigned at;
@@ -248,9 +277,8 @@ __global__ __launch_bounds__((WgShape<TM, TN>::T)) void q8_wgrad_kernel(Q8WgradA
       unsigned at;
       if constexpr (!ROWS) at = wg_piece((tid >> 3) + T / 8 * j, tid & 7);
       else at = wg_token<TN>(tid / (TN / 8) + T / (TN / 8) * j, tid % (TN / 8));
-      const unsigned w[2] = {rg.x[j].x, rg.x[j].y};
       float f[8];
-      q8_decode_vec<FMT, 8>(w, q8_scale(rg.s[j]), f);
+      q8_decode_vec<FMT, 8>(rg.x[j].w, q8_scale(rg.s[j]), f);
       *reinterpret_cast<csn_u4*>(bx + at) = wg_u4(wg_hi2(f[0], f[1]), wg_hi2(f[2], f[3]), wg_hi2(f[4], f[5]), wg_hi2(f[6], f[7]));
     }
   };
@@ -309,7 +337,7 @@ __global__ __launch_bounds__((WgShape<TM, TN>::T)) void q8_wgrad_kernel(Q8WgradA
   constexpr bool TWO = TM < 256;
   load(r0, s0);
   if constexpr (TWO) load(r1, s0 + 1);
-  store(r0, sm);
+  store(r0, s0, sm);
 #pragma unroll 1
   for (int s = s0; s < s1; s += 2) {
     const bool more = s + 2 < s1;
@@ -317,20 +345,20 @@ __global__ __launch_bounds__((WgShape<TM, TN>::T)) void q8_wgrad_kernel(Q8WgradA
       if (more) load(r0, s + 2);
       __syncthreads();
       multiply(sm);
-      store(r1, sm + BUF);
+      store(r1, s + 1, sm + BUF);
       if (more) load(r1, s + 3);
       __syncthreads();
       multiply(sm + BUF);
-      if (more) store(r0, sm);
+      if (more) store(r0, s + 2, sm);
     } else {
       load(r0, s + 1);
       __syncthreads();
       multiply(sm);
-      store(r0, sm + BUF);
+      store(r0, s + 1, sm + BUF);
       if (more) load(r0, s + 2);
       __syncthreads();
       multiply(sm + BUF);
-      if (more) store(r0, sm);
+      if (more) store(r0, s + 2, sm);
     }
   }
 
@@ -398,19 +426,19 @@ int64_t csn_q8_wgrad_partial_floats(int rows, int a16, int64_t outer, int64_t in
   return (int64_t)p.slabs * (cout * cin + cout);
 }
 
-template <typename AT, int FMT, bool ROWS, int TM, int TN>
-static int q8_wgrad_run(const Q8WgradArgs& a, void* stream) {
+template <typename AT, int FMT, bool ROWS, bool WIDE, int TM, int TN>
+static int q8_wgrad_go(const Q8WgradArgs& a, void* stream) {
   constexpr int smem = 2 * ((sizeof(AT) == 4 ? 3 : 1) * TM + TN) * WG_ROWB;
 #ifndef CSN_CPU_EMU
   static CsnPerDeviceOnce once;
   const int st = once.run([] {
-    return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(&q8_wgrad_kernel<AT, FMT, ROWS, TM, TN>),
+    return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(&q8_wgrad_kernel<AT, FMT, ROWS, WIDE, TM, TN>),
                                     hipFuncAttributeMaxDynamicSharedMemorySize, smem);
   });
   if (st != 0) return st;
 #endif
   const int total = a.mtiles * a.ntiles * a.slabs;
-  CSN_LAUNCH((q8_wgrad_kernel<AT, FMT, ROWS, TM, TN>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(WgShape<TM, TN>::T), smem, stream, a);
+  CSN_LAUNCH((q8_wgrad_kernel<AT, FMT, ROWS, WIDE, TM, TN>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(WgShape<TM, TN>::T), smem, stream, a);
   if (a.slabs > 1) {
     const int e = (int)hipGetLastError();
     if (e != 0) return e;
@@ -421,6 +449,12 @@ static int q8_wgrad_run(const Q8WgradArgs& a, void* stream) {
   return (int)hipGetLastError();
 }
 
+template <typename AT, int FMT, bool ROWS, int TM, int TN>
+static int q8_wgrad_run(const Q8WgradArgs& a, void* stream) {
+  if (ROWS ? a.cin >= 8 && a.cout >= 8 : a.inner >= 8) return q8_wgrad_go<AT, FMT, ROWS, true, TM, TN>(a, stream);
+  if constexpr (TM == 256) return -1;   // (never: that tile is for more channels)
+  else return q8_wgrad_go<AT, FMT, ROWS, false, TM, TN>(a, stream);
+}
 template <typename AT, int FMT, bool ROWS>
 static int q8_wgrad_tile(const Q8WgradArgs& a, const WgPlan& p, void* stream) {
   if constexpr (ROWS && sizeof(AT) == 2)
@@ -434,13 +468,10 @@ int csn_launch_q8_wgrad(const Q8WgradArgs& a0, int rows, int a16, int fmt, void*
   WgPlan p;
   if (!wg_plan(rows, a16, a.outer, a.inner, a.cin, a.cout, p)) return -1;
   a.mtiles = p.mtiles; a.ntiles = p.ntiles; a.steps = p.steps; a.steps_per_slab = p.steps_per_slab; a.slabs = p.slabs; a.chunks = p.chunks;
-  const uintptr_t py = (uintptr_t)a.dy, px = (uintptr_t)a.codes;
-  if (rows) {   // 8 channels of a token at once
-    a.vec_y = py % 16 == 0 && a.dy_so % 8 == 0;
-    a.vec_x = px % 8 == 0 && a.cin % 8 == 0;
-  } else {      // 8 pixels of a channel at once, no plane ending inside them
-    a.vec_y = a.inner % 8 == 0 && py % 16 == 0 && a.dy_so % 8 == 0 && a.dy_sc % 8 == 0;
-    a.vec_x = a.inner % 8 == 0 && px % 8 == 0;
+  if (a.outer * a.inner == 0) {   // no tokens: the gradients are zero
+    SlabSumArgs r;
+    r.partial = nullptr; r.out0 = a.dweight; r.out1 = a.dbias; r.n0 = a.cout * a.cin; r.n = r.n0 + a.cout; r.slabs = 0;
+    return csn_launch_slab_sum(r, stream);
   }
   if (fmt == Q8_INT8) {
     if (rows) return a16 ? q8_wgrad_tile<csn_bf16, Q8_INT8, true>(a, p, stream) : q8_wgrad_tile<float, Q8_INT8, true>(a, p, stream);
