@@ -177,12 +177,12 @@ __global__ __launch_bounds__(NormRowsBlock<G>::T) void norm_rows_fwd_kernel(Norm
 #pragma unroll
     for (int v = 0; v < NV; ++v) vec_load<W>(nx[v], x + E * (l + G * v), n[v]);
   };
-  if (t < a.outer) load(t);
+  load(t < a.outer ? t : a.outer - 1);
   for (; t < a.outer; t += step) {
     VecIo<AT> r[NV];
 #pragma unroll
     for (int v = 0; v < NV; ++v) r[v] = nx[v];
-    if (t + step < a.outer) load(t + step);   // (in flight while this token is worked on)
+    load(t + step < a.outer ? t + step : a.outer - 1);   // (in flight while this token is worked on; a branch around it would be a wait)
     float s[1] = {0.f};
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -283,14 +283,14 @@ __global__ __launch_bounds__(NormRowsBlock<G>::T) void norm_rows_bwd_kernel(Norm
     }
     nmean = a.mean[row]; nrstd = a.rstd[row];
   };
-  if (t < a.outer) load(t);
+  load(t < a.outer ? t : a.outer - 1);
   for (; t < a.outer; t += step) {
     NormIn<AT, E, SRC> rx[NV];
     VecIo<AT> rd[NV];
 #pragma unroll
     for (int v = 0; v < NV; ++v) { rx[v] = nx[v]; rd[v] = nd[v]; }
     const float mean = nmean, rstd = nrstd;
-    if (t + step < a.outer) load(t + step);   // (in flight while this token is worked on)
+    load(t + step < a.outer ? t + step : a.outer - 1);   // (in flight while this token is worked on; a branch around it would be a wait)
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -547,7 +547,7 @@ __global__ __launch_bounds__(T) void norm_planar_bwd_kernel(NormArgs a) {
     vec_load<true>(nm, a.mean + st, n);
     vec_load<true>(nr, a.rstd + st, n);
   };
-  if ((int)blockIdx.x < a.items) load(blockIdx.x);
+  load(min((int)blockIdx.x, a.items - 1));
   for (int it = blockIdx.x; it < a.items; it += gridDim.x) {
     const int o = it / a.tiles, t0 = (it - o * a.tiles) * TP;
     const int n = P - t0 - px * E;
@@ -558,7 +558,7 @@ __global__ __launch_bounds__(T) void norm_planar_bwd_kernel(NormArgs a) {
     VecIo<float> cm = nm, cr = nr;
 #pragma unroll
     for (int k = 0; k < NC; ++k) { rx[k] = nx[k]; rd[k] = nd[k]; }
-    if (it + (int)gridDim.x < a.items) load(it + gridDim.x);   // (in flight while this tile is worked on)
+    load(min(it + (int)gridDim.x, a.items - 1));   // (in flight while this tile is worked on; a branch around it would be a wait)
     if (t0 + TP > P) {   // (the image's last tile, one branch for all channels: the sums below stay one straight block)
       vec_end<true>(cm, n);
       vec_end<true>(cr, n);

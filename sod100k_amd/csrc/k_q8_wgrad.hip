@@ -7,10 +7,11 @@
 // v_mfma_f32_32x32x16_bf16 as it is.  A float dY is cut by truncation into three bfloat16 numbers of 8 bits each (exact), whose
 // products with X go into the same accumulators: three matrix instructions, nothing lost but the accumulation's own rounding.
 //
-// Block = TM x TN of dW over a slab of the tokens.  64 tokens are staged at a time into two LDS buffers.
-// Planar maps hold eight consecutive pixels of a channel together, an operand of the matrix instruction: LDS rows are channels, [row][64
-// tokens], operands are 128-bit reads.  The 16-byte piece c of row r lies at c ^ f(r), f(r) = (r ^ r >> 3) & 7, so that eight consecutive
-// rows fall on eight different pieces.
+// Block = TM x TN of dW over a slab of the tokens.  64 tokens -- 128 of bfloat16 maps, whose codes then come by whole lines -- are staged at a
+// time into two LDS buffers.
+// Planar maps hold eight consecutive pixels of a channel together, an operand of the matrix instruction: LDS rows are channels,
+// [row][tokens], operands are 128-bit reads.  The 16-byte piece c of row r lies at c ^ (r & 7), so that eight consecutive rows fall on eight
+// different pieces.
 // Token rows hold the channels of a token together: LDS rows are tokens, [64 tokens][row], as they come, and the operands -- eight
 // tokens of a channel -- are formed by the transposing LDS read, four tokens of 16 channels per 16 lanes.  Its four rows' 32 bytes
 // lie in different banks: the 16-byte pieces of token t are exchanged by an xor with 2 (t & 7).
@@ -27,10 +28,8 @@ int csn_launch_q8_wgrad(const Q8WgradArgs&, int, int, int, void*) { return -1; }
 int64_t csn_q8_wgrad_partial_floats(int, int, int64_t, int64_t, int64_t, int64_t) { return 0; }
 #else
 
-#define WG_STEP 64      // tokens of a step
-#define WG_ROWB 128     // bytes of a staged row
-
-__device__ __forceinline__ unsigned wg_piece(int row, int c) { return (unsigned)(row * WG_ROWB + ((c ^ ((row ^ (row >> 3)) & 7)) << 4)); }
+template <int STEP>   // planar: channel rows of STEP tokens
+__device__ __forceinline__ unsigned wg_piece(int row, int c) { return (unsigned)(row * (2 * STEP) + ((c ^ (row & 7)) << 4)); }
 template <int C>   // token rows of C channels
 __device__ __forceinline__ unsigned wg_token(int t, int piece) {
   constexpr int M = C >= 128 ? 7 : 3;
@@ -101,10 +100,13 @@ template <> struct WgY<float> {
   }
 };
 
-// waves of a block and their grid over its tile: 64 x 64 .. 128 x 128 on four waves (2 x 2), 256 x 256 on eight (2 x 4)
-template <int TM, int TN> struct WgShape {
-  static constexpr int T = TM == 256 ? 512 : 256, WM = 2, WN = T / 64 / WM;
+// tokens of a step; waves of a block and their grid over its tile
+template <typename AT, bool ROWS, int TM, int TN> struct WgShape {
+  static constexpr int STEP = !ROWS && sizeof(AT) == 2 ? 128 : 64;
+  static constexpr int T = TM == 256 || (STEP == 128 && TM + TN > 128) ? 512 : 256;
+  static constexpr int WM = T == 512 && TM > TN ? 4 : 2, WN = T / 64 / WM;
   static constexpr int MI = TM / WM / 32, NJ = TN / WN / 32;      // 32 x 32 tiles of a wave
+  static constexpr int SMEM = 2 * ((sizeof(AT) == 4 ? 3 : 1) * TM + TN) * 2 * STEP;
 };
 // what a thread holds of a step in flight: pieces of eight elements of dY and of X (planar: n pixels of each are the map's)
 template <typename AT, int NY, int NX> struct WgRegs {
@@ -118,12 +120,13 @@ template <typename AT, int NY, int NX> struct WgRegs {
 // and shifted (vec_io.h); channels past the last one are loaded from inside the tensor -- every entry of dW is a sum of its own and
 // those are not stored -- and only tokens past the last one are cleared.
 template <typename AT, int FMT, bool ROWS, bool WIDE, int TM, int TN>
-__global__ __launch_bounds__((WgShape<TM, TN>::T)) void q8_wgrad_kernel(Q8WgradArgs a) {
+__global__ __launch_bounds__((WgShape<AT, ROWS, TM, TN>::T)) void q8_wgrad_kernel(Q8WgradArgs a) {
   CSN_DYN_SMEM(unsigned char, sm);
-  typedef WgShape<TM, TN> S;
-  constexpr int PARTS = sizeof(AT) == 4 ? 3 : 1, T = S::T, MI = S::MI, NJ = S::NJ;
-  constexpr unsigned YB = TM * WG_ROWB, BUF = PARTS * YB + TN * WG_ROWB;   // (64 tokens x TM bfloat16 either way)
-  constexpr int NY = TM * 8 / T, NX = TN * 8 / T;                          // pieces per thread and step
+  typedef WgShape<AT, ROWS, TM, TN> S;
+  constexpr int PARTS = sizeof(AT) == 4 ? 3 : 1, T = S::T, MI = S::MI, NJ = S::NJ, STEP = S::STEP;
+  constexpr unsigned YB = TM * 2 * STEP, BUF = PARTS * YB + TN * 2 * STEP;   // (STEP tokens x TM bfloat16 either way)
+  constexpr int NY = TM * (STEP / 8) / T, NX = TN * (STEP / 8) / T;          // pieces per thread and step
+  constexpr int PP = STEP / 8, PR = T / PP;                                  // planar: pieces of a channel, channels a load round covers
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   // (slab, tile) items in order over the XCDs (block b runs on XCD b % 8): the tiles of a slab read the same tokens, through one L2
   const int ntile = a.mtiles * a.ntiles, total = ntile * a.slabs, per = (total + 7) >> 3;
@@ -141,8 +144,8 @@ __global__ __launch_bounds__((WgShape<TM, TN>::T)) void q8_wgrad_kernel(Q8WgradA
   WgRegs<AT, NY, NX> r0, r1;
 
   auto load = [&](WgRegs<AT, NY, NX>& rg, int step) {
-    if constexpr (!ROWS) {   // piece j: channel (tid >> 3) + j T / 8, eight pixels number tid & 7 of the step
-      const unsigned g = (unsigned)step * 8u + (unsigned)(tid & 7);
+    if constexpr (!ROWS) {   // piece j: channel tid / PP + j PR, eight pixels number tid % PP of the step
+      const unsigned g = (unsigned)step * PP + (unsigned)(tid % PP);
       unsigned o = g / (unsigned)a.chunks, c = g - o * (unsigned)a.chunks;
       const bool in = (int64_t)o < a.outer;
       if (!in) { o = (unsigned)a.outer - 1; c = 0; }
@@ -154,23 +157,23 @@ __global__ __launch_bounds__((WgShape<TM, TN>::T)) void q8_wgrad_kernel(Q8WgradA
       if constexpr (WIDE) {
         py -= 8 - left;
 #pragma unroll
-        for (int j = 0; j < NY; ++j) rg.y[j].load(py + (int64_t)min((int64_t)(o0 + (tid >> 3) + T / 8 * j), a.cout - 1) * a.dy_sc);
+        for (int j = 0; j < NY; ++j) rg.y[j].load(py + (int64_t)min((int64_t)(o0 + tid / PP + PR * j), a.cout - 1) * a.dy_sc);
 #pragma unroll
         for (int j = 0; j < NX; ++j) {
-          const int64_t row = row0 + min((int64_t)(i0 + (tid >> 3) + T / 8 * j), a.cin - 1);
+          const int64_t row = row0 + min((int64_t)(i0 + tid / PP + PR * j), a.cin - 1);
           rg.x[j].load(a.codes + row * a.inner + p - (8 - left));
           rg.s[j] = a.exps[row * a.nblk + (p >> 5)];
         }
       } else {
 #pragma unroll
         for (int j = 0; j < NY; ++j) {
-          const int r = o0 + (tid >> 3) + T / 8 * j;
+          const int r = o0 + tid / PP + PR * j;
           rg.y[j].zero();
           if (r < a.cout) rg.y[j].load_each(py + (int64_t)r * a.dy_sc, n);
         }
 #pragma unroll
         for (int j = 0; j < NX; ++j) {
-          const int r = i0 + (tid >> 3) + T / 8 * j;
+          const int r = i0 + tid / PP + PR * j;
           rg.x[j].zero();
           rg.s[j] = 127;
           if (r < a.cin && n > 0) {
@@ -181,7 +184,7 @@ __global__ __launch_bounds__((WgShape<TM, TN>::T)) void q8_wgrad_kernel(Q8WgradA
       }
     } else {                 // piece j: token tid / (TM / 8) + j T / (TM / 8) of the step, eight channels number tid % (TM / 8)
       constexpr int GY = TM / 8, GX = TN / 8;
-      const int64_t t0 = (int64_t)step * WG_STEP;
+      const int64_t t0 = (int64_t)step * STEP;
       const int cy = o0 + 8 * (tid % GY), cx = i0 + 8 * (tid % GX);
       if constexpr (WIDE) {
         const int by = min(cy, (int)a.cout - 8), bx = min(cx, (int)a.cin - 8);   // (stepped back; wholly outside: anywhere)
@@ -233,7 +236,7 @@ __global__ __launch_bounds__((WgShape<TM, TN>::T)) void q8_wgrad_kernel(Q8WgradA
     }
     if constexpr (WIDE && ROWS) {
       constexpr int GY = TM / 8, GX = TN / 8;
-      const int64_t t0 = (int64_t)step * WG_STEP;
+      const int64_t t0 = (int64_t)step * STEP;
       const int cy = o0 + 8 * (tid % GY), cx = i0 + 8 * (tid % GX);
       if (o0 + TM > a.cout && cy < a.cout && cy + 8 > a.cout)
 #pragma unroll
@@ -241,7 +244,7 @@ __global__ __launch_bounds__((WgShape<TM, TN>::T)) void q8_wgrad_kernel(Q8WgradA
       if (i0 + TN > a.cin && cx < a.cin && cx + 8 > a.cin)
 #pragma unroll
         for (int j = 0; j < NX; ++j) code_end<true, 8>(rg.x[j], (int)a.cin - cx);
-      if (t0 + WG_STEP > a.outer) {
+      if (t0 + STEP > a.outer) {
 #pragma unroll
         for (int j = 0; j < NY; ++j)
           if (t0 + tid / GY + T / GY * j >= a.outer) rg.y[j].zero();
@@ -258,7 +261,7 @@ __global__ __launch_bounds__((WgShape<TM, TN>::T)) void q8_wgrad_kernel(Q8WgradA
 #pragma unroll
     for (int j = 0; j < NY; ++j) {
       unsigned at;
-      if constexpr (!ROWS) at = wg_piece((tid >> 3) + T / 8 * j, tid & 7);
+      if constexpr (!ROWS) at = wg_piece<STEP>(tid / PP + PR * j, tid % PP);
       else at = wg_token<TM>(tid / (TM / 8) + T / (TM / 8) * j, tid % (TM / 8));
       rg.y[j].put(buf, at, YB);
       if (bias) {
@@ -275,7 +278,7 @@ __global__ __launch_bounds__((WgShape<TM, TN>::T)) void q8_wgrad_kernel(Q8WgradA
 #pragma unroll
     for (int j = 0; j < NX; ++j) {
       unsigned at;
-      if constexpr (!ROWS) at = wg_piece((tid >> 3) + T / 8 * j, tid & 7);
+      if constexpr (!ROWS) at = wg_piece<STEP>(tid / PP + PR * j, tid % PP);
       else at = wg_token<TN>(tid / (TN / 8) + T / (TN / 8) * j, tid % (TN / 8));
       float f[8];
       q8_decode_vec<FMT, 8>(rg.x[j].w, q8_scale(rg.s[j]), f);
@@ -311,12 +314,12 @@ __global__ __launch_bounds__((WgShape<TM, TN>::T)) void q8_wgrad_kernel(Q8WgradA
   };
   auto multiply = [&](const unsigned char* buf) {
 #pragma unroll
-    for (int kk = 0; kk < WG_STEP / 16; ++kk) {
+    for (int kk = 0; kk < STEP / 16; ++kk) {
       csn_u4 b[NJ];
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         if constexpr (ROWS) b[j] = read8(buf + xa[j][0] + 32 * TN * kk, buf + xa[j][1] + 32 * TN * kk);
-        else b[j] = *reinterpret_cast<const csn_u4*>(buf + PARTS * YB + wg_piece(wc + 32 * j + (lane & 31), 2 * kk + (lane >> 5)));
+        else b[j] = *reinterpret_cast<const csn_u4*>(buf + PARTS * YB + wg_piece<STEP>(wc + 32 * j + (lane & 31), 2 * kk + (lane >> 5)));
       }
 #pragma unroll
       for (int part = 0; part < PARTS; ++part)
@@ -324,7 +327,7 @@ __global__ __launch_bounds__((WgShape<TM, TN>::T)) void q8_wgrad_kernel(Q8WgradA
         for (int i = 0; i < MI; ++i) {
           csn_u4 y;
           if constexpr (ROWS) y = read8(buf + part * YB + ya[i][0] + 32 * TM * kk, buf + part * YB + ya[i][1] + 32 * TM * kk);
-          else y = *reinterpret_cast<const csn_u4*>(buf + part * YB + wg_piece(wr + 32 * i + (lane & 31), 2 * kk + (lane >> 5)));
+          else y = *reinterpret_cast<const csn_u4*>(buf + part * YB + wg_piece<STEP>(wr + 32 * i + (lane & 31), 2 * kk + (lane >> 5)));
 #pragma unroll
           for (int j = 0; j < NJ; ++j) acc[i][j] = csn_mfma_32x32x16_bf16(y, b[j], acc[i][j]);
         }
@@ -334,33 +337,31 @@ __global__ __launch_bounds__((WgShape<TM, TN>::T)) void q8_wgrad_kernel(Q8WgradA
   // The slab's steps in pairs (steps_per_slab is even, tokens behind the last read as zeros).  Two register sets: the registers of a step
   // are free again once it lies in its buffer, and hold the step two further on while the buffers are multiplied.  The large tile's
   // accumulators leave room for one set, one step ahead.
+  // (The last pair stands by itself: loads behind a branch would be waited for where the paths join again.)
   constexpr bool TWO = TM < 256;
   load(r0, s0);
   if constexpr (TWO) load(r1, s0 + 1);
   store(r0, s0, sm);
 #pragma unroll 1
-  for (int s = s0; s < s1; s += 2) {
-    const bool more = s + 2 < s1;
-    if constexpr (TWO) {
-      if (more) load(r0, s + 2);
-      __syncthreads();
-      multiply(sm);
-      store(r1, s + 1, sm + BUF);
-      if (more) load(r1, s + 3);
-      __syncthreads();
-      multiply(sm + BUF);
-      if (more) store(r0, s + 2, sm);
-    } else {
-      load(r0, s + 1);
-      __syncthreads();
-      multiply(sm);
-      store(r0, s + 1, sm + BUF);
-      if (more) load(r0, s + 2);
-      __syncthreads();
-      multiply(sm + BUF);
-      if (more) store(r0, s + 2, sm);
-    }
+  for (int s = s0; s + 2 < s1; s += 2) {
+    load(r0, s + (TWO ? 2 : 1));
+    __syncthreads();
+    multiply(sm);
+    if constexpr (TWO) store(r1, s + 1, sm + BUF);
+    else store(r0, s + 1, sm + BUF);
+    if constexpr (TWO) load(r1, s + 3);
+    else load(r0, s + 2);
+    __syncthreads();
+    multiply(sm + BUF);
+    store(r0, s + 2, sm);
   }
+  if constexpr (!TWO) load(r0, s1 - 1);
+  __syncthreads();
+  multiply(sm);
+  if constexpr (TWO) store(r1, s1 - 1, sm + BUF);
+  else store(r0, s1 - 1, sm + BUF);
+  __syncthreads();
+  multiply(sm + BUF);
 
   float* out = a.slabs > 1 ? a.partial + (int64_t)slab * a.cout * (a.cin + 1) : a.dweight;
 #pragma unroll
@@ -376,12 +377,12 @@ __global__ __launch_bounds__((WgShape<TM, TN>::T)) void q8_wgrad_kernel(Q8WgradA
         }
     }
   if (bias) {   // the block's sums of dY: K threads hold a channel's
-    constexpr int K = ROWS ? T / (TM / 8) : 8;
+    constexpr int K = ROWS ? T / (TM / 8) : PP;
     __syncthreads();
     float* sb = reinterpret_cast<float*>(sm);   // [TM][K]
     if constexpr (!ROWS) {
 #pragma unroll
-      for (int j = 0; j < NY; ++j) sb[((tid >> 3) + T / 8 * j) * K + (tid & 7)] = bsum[j];
+      for (int j = 0; j < NY; ++j) sb[(tid / PP + PR * j) * K + tid % PP] = bsum[j];
     } else {
 #pragma unroll
       for (int q = 0; q < 8; ++q) sb[(8 * (tid % (TM / 8)) + q) * K + tid / (TM / 8)] = bsum[q];
@@ -395,28 +396,26 @@ __global__ __launch_bounds__((WgShape<TM, TN>::T)) void q8_wgrad_kernel(Q8WgradA
   }
 }
 
-struct WgPlan { int tm, tn, mtiles, ntiles, steps, steps_per_slab, slabs, chunks; };
+struct WgPlan { int tm, tn, mtiles, ntiles, steps_per_slab, slabs, chunks; };
 
 // Tiles of 128 where the channels fill more than 64; of 256 x 256, whose operands are read from LDS half as often, where there are enough of
-// them times steps for every CU (bfloat16 dY: the three parts of a float one do not fit).  About two blocks per CU -- one of the large tile --
-// but at least four steps of 64 tokens each: a slab costs a partial tile written and read again.
+// them times steps for every CU (bfloat16 dY: the three parts of a float one do not fit).  About one block of eight waves or two of four
+// per CU, but at least 256 tokens each: a slab costs a partial tile written and read again.
 static bool wg_plan(int rows, int a16, int64_t outer, int64_t inner, int64_t cin, int64_t cout, WgPlan& p) {
-  const int64_t chunks = rows ? 1 : (inner + 7) / 8;
-  const int64_t all = rows ? (outer + 7) / 8 : outer * chunks, steps = (all + 7) / 8;
+  const int64_t chunks = rows ? 1 : (inner + 7) / 8, per_step = !rows && a16 ? 16 : 8;
+  const int64_t all = rows ? (outer + 7) / 8 : outer * chunks, steps = (all + per_step - 1) / per_step;
   p.tm = cout > 64 ? 128 : 64;
   p.tn = cin > 64 ? 128 : 64;
   const bool big = rows && a16 && cout > 128 && cin > 128 && ((cout + 255) / 256) * ((cin + 255) / 256) * steps >= 256 * 8;
   if (big) p.tm = p.tn = 256;
   const int64_t mt = (cout + p.tm - 1) / p.tm, nt = (cin + p.tn - 1) / p.tn;
-  if (mt * nt > (1 << 20) || all > 0x7ffffff0LL || chunks > 0x7ffffff0LL) return false;
-  int64_t slabs = ((big ? 256 : 512) + mt * nt - 1) / (mt * nt);
-  slabs = std::min(slabs, (steps + 3) / 4);
-  if (slabs < 1) slabs = 1;
-  p.mtiles = (int)mt; p.ntiles = (int)nt; p.steps = (int)steps; p.chunks = (int)(chunks < 1 ? 1 : chunks);
-  p.steps_per_slab = ((int)((steps + slabs - 1) / slabs) + 1) & ~1;
-  if (p.steps_per_slab < 2) p.steps_per_slab = 2;
-  p.slabs = (int)((steps + p.steps_per_slab - 1) / p.steps_per_slab);
-  if (p.slabs < 1) p.slabs = 1;
+  if (mt * nt > (1 << 20) || all > 0x7ffffe00LL || chunks > 0x7ffffe00LL) return false;
+  const bool eight = big || (per_step == 16 && p.tm + p.tn > 128);
+  int64_t slabs = ((eight ? 256 : 512) + mt * nt - 1) / (mt * nt);
+  slabs = std::max(std::min(slabs, (steps * per_step + 31) / 32), (int64_t)1);
+  p.mtiles = (int)mt; p.ntiles = (int)nt; p.chunks = (int)std::max(chunks, (int64_t)1);
+  p.steps_per_slab = std::max(((int)((steps + slabs - 1) / slabs) + 1) & ~1, 2);
+  p.slabs = std::max((int)((steps + p.steps_per_slab - 1) / p.steps_per_slab), 1);
   return true;
 }
 
@@ -428,17 +427,17 @@ int64_t csn_q8_wgrad_partial_floats(int rows, int a16, int64_t outer, int64_t in
 
 template <typename AT, int FMT, bool ROWS, bool WIDE, int TM, int TN>
 static int q8_wgrad_go(const Q8WgradArgs& a, void* stream) {
-  constexpr int smem = 2 * ((sizeof(AT) == 4 ? 3 : 1) * TM + TN) * WG_ROWB;
+  typedef WgShape<AT, ROWS, TM, TN> S;
 #ifndef CSN_CPU_EMU
   static CsnPerDeviceOnce once;
   const int st = once.run([] {
     return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(&q8_wgrad_kernel<AT, FMT, ROWS, WIDE, TM, TN>),
-                                    hipFuncAttributeMaxDynamicSharedMemorySize, smem);
+                                    hipFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
   });
   if (st != 0) return st;
 #endif
   const int total = a.mtiles * a.ntiles * a.slabs;
-  CSN_LAUNCH((q8_wgrad_kernel<AT, FMT, ROWS, WIDE, TM, TN>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(WgShape<TM, TN>::T), smem, stream, a);
+  CSN_LAUNCH((q8_wgrad_kernel<AT, FMT, ROWS, WIDE, TM, TN>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(S::T), S::SMEM, stream, a);
   if (a.slabs > 1) {
     const int e = (int)hipGetLastError();
     if (e != 0) return e;
@@ -467,7 +466,7 @@ int csn_launch_q8_wgrad(const Q8WgradArgs& a0, int rows, int a16, int fmt, void*
   Q8WgradArgs a = a0;
   WgPlan p;
   if (!wg_plan(rows, a16, a.outer, a.inner, a.cin, a.cout, p)) return -1;
-  a.mtiles = p.mtiles; a.ntiles = p.ntiles; a.steps = p.steps; a.steps_per_slab = p.steps_per_slab; a.slabs = p.slabs; a.chunks = p.chunks;
+  a.mtiles = p.mtiles; a.ntiles = p.ntiles; a.steps_per_slab = p.steps_per_slab; a.slabs = p.slabs; a.chunks = p.chunks;
   if (a.outer * a.inner == 0) {   // no tokens: the gradients are zero
     SlabSumArgs r;
     r.partial = nullptr; r.out0 = a.dweight; r.out1 = a.dbias; r.n0 = a.cout * a.cin; r.n = r.n0 + a.cout; r.slabs = 0;

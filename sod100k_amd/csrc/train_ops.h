@@ -78,7 +78,7 @@ struct Q8WgradArgs {
   int64_t dy_so, dy_sc;
   int64_t nblk;             // checkpoint blocks of a plane / row
   // set by the launcher
-  int32_t mtiles, ntiles, slabs, steps, steps_per_slab, chunks;   // chunks: 8-pixel pieces of a plane
+  int32_t mtiles, ntiles, slabs, steps_per_slab, chunks;   // chunks: 8-pixel pieces of a plane
 };
 int csn_launch_q8_wgrad(const Q8WgradArgs& a, int rows, int a16, int fmt, void* stream);
 int64_t csn_q8_wgrad_partial_floats(int rows, int a16, int64_t outer, int64_t inner, int64_t cin, int64_t cout);
