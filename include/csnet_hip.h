@@ -231,7 +231,8 @@ int csn_adam_step(float* p, const float* g, float* m, float* v, const float* wd,
  * Layouts.  CSN_LAYOUT_PLANAR: [outer][channels][inner], the framework's planar maps, one token per pixel.
  * CSN_LAYOUT_ROWS: [outer][channels], one token per row, inner = 1.  Inputs may be slices of wider tensors: element (o, c, p) lies
  * at o * outer_stride + c * channel_stride + p (planar), o * outer_stride + c (rows; channel_stride is ignored); strides count
- * elements and may be zero (broadcast).  Outputs are dense, weights and their gradients float.
+ * elements and may be zero (broadcast).  Outputs are dense and overlap neither each other nor the inputs; weights and their gradients
+ * are float.
  *
  * 8-bit checkpoint of a tensor (CSN_Q8_INT8 / CSN_Q8_E4M3): the elements of a plane (planar) or of a row (rows) in blocks of 32,
  * the last block of each short; one byte of exponent s per block, one byte of code per element:
@@ -287,7 +288,8 @@ typedef struct csn_product_desc {
 
 /* Weight and bias gradient of y[t] = W x[t] + b (a 1x1 convolution over planar maps, a linear layer over rows) from the checkpoint
  * of x:  dweight[o][i] = sum_t dy[t][o] value(x[t][i]),  dbias[o] = sum_t dy[t][o]  (WRITTEN; dbias may be null).  bfloat16 dy
- * and the values are multiplied exactly on the matrix cores, float dy as three bfloat16 parts (all 24 bits). */
+ * and the values are multiplied exactly on the matrix cores, float dy as three bfloat16 parts (all 24 bits).  Infinities and NaN of dy
+ * or x stay in the entries that they reach; an infinite float dy may give NaN there. */
 size_t csn_product_weight_grad_workspace_bytes(const csn_product_desc* d);
 int csn_product_weight_grad(const csn_product_desc* d, const void* dy, int64_t dy_outer_stride, int64_t dy_channel_stride,
                             const uint8_t* codes, const uint8_t* exponents, float* dweight, float* dbias, void* workspace,

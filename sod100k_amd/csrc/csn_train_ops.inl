@@ -74,7 +74,7 @@ int64_t plan_saved_bytes(const csn_plan* P) {
              [&](int64_t, int64_t bytes) { n += align_up(bytes, 256); });
   return n;
 }
-int plan_saved_move(csn_plan* P, char* ws, char* ck, int format, bool pack, void* stream) {
+int plan_saved_move(csn_plan* P, char* ws, char* ck, int format, bool pack, void* stream) try {
   std::vector<Q8Seg> qs;
   std::vector<CopySeg> cs;
   int64_t at = 0;
@@ -96,6 +96,8 @@ int plan_saved_move(csn_plan* P, char* ws, char* ck, int format, bool pack, void
   LAUNCH_TRY(csn_launch_q8_segments(qs.data(), (int)qs.size(), pack, P->act16 ? 1 : 0, format, stream));
   LAUNCH_TRY(csn_launch_copy_segments(cs.data(), (int)cs.size(), stream));
   return CSN_OK;
+} catch (const std::bad_alloc&) {
+  REFUSE("plan checkpoint: out of host memory");
 }
 
 }  // namespace

@@ -624,7 +624,7 @@ class _CSNetTrainFn(torch.autograd.Function):
         ctx.model, ctx.x = model, x
         fmt = getattr(model, "_train_checkpoints", None)
         if fmt is not None:
-            ctx.saved = _SavedForward(model.engine_for(x, train=True), {"int8": N.Q8_INT8, "e4m3": N.Q8_E4M3}[fmt], model._flop_tab)
+            ctx.saved = _SavedForward(model, x, {"int8": N.Q8_INT8, "e4m3": N.Q8_E4M3}[fmt])
         else:
             ctx.saved = None
         # backward reads z / activations / BN statistics of THIS forward from the plan's workspace: remember which
@@ -663,6 +663,8 @@ class _CSNetTrainFn(torch.autograd.Function):
         its checkpoint."""
         model, s = ctx.model, ctx.saved
         eng, arena = s.engine, model._arena
+        if s.versions != _versions(model):
+            raise RuntimeError("CSNet backward after an in-place change of the parameters: its gradients are those of the forward's")
         if eng.waiting is not None and eng.waiting() is s:
             pass
         elif s.checkpoint is not None:
@@ -670,6 +672,7 @@ class _CSNetTrainFn(torch.autograd.Function):
             if waiting is not None:                     # the workspace holds another forward that still waits: out of the way
                 waiting.checkpoint = eng.checkpoint_save(waiting.format)
             eng.checkpoint_restore(s.checkpoint, s.format)
+            model._train_generation += 1                # (a forward without checkpoints in between is gone, too)
         else:
             raise RuntimeError("CSNet backward a second time through one forward: its saved tensors are gone")
         eng.waiting = None                              # csn_backward writes over them
@@ -688,9 +691,15 @@ class _SavedForward:
     """A train-mode forward that waits for its backward (set_train_checkpoints): the plan that ran it and, once another forward
     needed that plan's workspace, its 8-bit checkpoint.  The plan refers to it weakly: a graph that was dropped saves nothing."""
 
-    def __init__(self, engine, format, flop_tab):
-        self.engine, self.format, self.flop_tab, self.checkpoint = engine, format, flop_tab, None
-        engine.waiting = weakref.ref(self)
+    def __init__(self, model, x, format):
+        self.engine, self.format, self.flop_tab, self.checkpoint = model.engine_for(x, train=True), format, model._flop_tab, None
+        self.versions = _versions(model)
+        self.engine.waiting = weakref.ref(self)
+
+
+def _versions(model):
+    """What in-place changes of the parameters by torch move (a forward that waits must not see any)."""
+    return [p._version for p in model.parameters()]
 
 
 # ---- dynamic weight decay hook (csnet.py:391-410) -----------------------------------------------------------

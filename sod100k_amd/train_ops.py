@@ -165,13 +165,15 @@ def _param(t: Optional[torch.Tensor], channels: int, what: str) -> Optional[torc
 
 
 def _norm_desc(rows: bool, dt: int, shape, eps: float, fmt: int) -> N.NormDesc:
-    d = N.NormDesc()
-    d.layout, d.dtype, d.eps, d.format = (N.LAYOUT_ROWS if rows else N.LAYOUT_PLANAR), dt, float(eps), fmt
     if rows:
-        d.outer, d.channels, d.inner = math.prod(shape[:-1]), shape[-1], 1
-    else:
-        d.outer, d.channels, d.inner = shape[0], shape[1], math.prod(shape[2:])
-    return d
+        return N.NormDesc(N.LAYOUT_ROWS, dt, math.prod(shape[:-1]), shape[-1], 1, eps, fmt)
+    return N.NormDesc(N.LAYOUT_PLANAR, dt, shape[0], shape[1], math.prod(shape[2:]), eps, fmt)
+
+
+def _dense_like(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+
+
 
 
 def layer_norm_forward(lib: C.CDLL, x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -187,10 +189,9 @@ def layer_norm_forward(lib: C.CDLL, x: torch.Tensor, weight: Optional[torch.Tens
     dev = _same_device(lib, x, weight, bias)
     fmt = _format(checkpoint) if checkpoint is not None else 0
     d = _norm_desc(rows, dt, x.shape, eps, fmt)
-    y = x.new_empty(x.shape)
+    y = _dense_like(x)
     sshape = x.shape[:-1] if rows else x.shape[:1] + x.shape[2:]
-    mean = x.new_empty(sshape, dtype=torch.float32)
-    rstd = x.new_empty(sshape, dtype=torch.float32)
+    mean, rstd = x.new_empty((2,) + sshape, dtype=torch.float32).unbind()   # (one allocation: the host's share of a small call)
     q = codes = scales = None
     if checkpoint is not None:
         start = -1 if rows else 2
@@ -228,7 +229,7 @@ def layer_norm_backward(lib: C.CDLL, dy: torch.Tensor, x: Union[torch.Tensor, Q8
     mean, rstd = mean.contiguous(), rstd.contiguous()
     dev = _same_device(lib, dy, src, q.scales if q is not None else None, mean, rstd, weight)
     d = _norm_desc(rows, dt, dy.shape, 1.0, fmt)
-    dx = dy.new_empty(dy.shape)
+    dx = _dense_like(dy)
     dweight = dy.new_empty((ch,), dtype=torch.float32)
     dbias = dy.new_empty((ch,), dtype=torch.float32)
     nbytes = lib.csn_layer_norm_workspace_bytes(C.byref(d))

@@ -242,3 +242,7 @@ def test_gpu_plan_checkpoint(lib, x2_manifest, act_dtype, fmt):
 @pytest.mark.parametrize("act_dtype,fmt", [("fp32", "e4m3"), ("bf16", "int8")])
 def test_gpu_two_forwards_one_backward(lib, x2_manifest, act_dtype, fmt):
     K.check_two_forwards_one_backward(lib, torch.device(DEV), x2_manifest, act_dtype, fmt, B=2, size=48)
+
+
+def test_gpu_waiting_forwards_refuse(lib, x2_manifest):
+    K.check_waiting_forwards_refuse(lib, torch.device(DEV), x2_manifest, B=2, size=48)

@@ -115,6 +115,10 @@ def test_emu_two_forwards_one_backward(lib, x2_manifest):
     K.check_two_forwards_one_backward(lib, torch.device("cpu"), x2_manifest, "fp32", "int8", size=16, quick=True)
 
 
+def test_emu_waiting_forwards_refuse(lib, x2_manifest):
+    K.check_waiting_forwards_refuse(lib, torch.device("cpu"), x2_manifest)
+
+
 def test_plan_checkpoint_refusals(lib, x2_manifest):
     import parity_cases as P
     m, _ = P.make_model(lib, x2_manifest, torch.device("cpu"))

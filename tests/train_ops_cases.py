@@ -10,6 +10,7 @@ CHAIN = 1024 for the sums over tokens."""
 import ctypes as C
 import math
 
+import pytest
 import torch
 
 from sod100k_amd import _native as N, train_ops as T
@@ -604,3 +605,23 @@ def check_two_forwards_one_backward(lib, device, manifest, act_dtype, fmt, B=2, 
     assert m.engine_for(xs[1], train=True).waiting().checkpoint is None
     b.backward(dy)
     assert torch.equal(flat(m), exact1)
+
+
+def check_waiting_forwards_refuse(lib, device, manifest, B=1, size=16):
+    """Backwards whose forward's tensors or parameters are no longer there: refused, never wrong."""
+    from oracle import inputs as I
+    xs = [torch.from_numpy(I.randn_batch(s, B, size, size)).to(device) for s in (31, 32)]
+    m = _net(lib, device, manifest, "fp32", B)
+    m.set_train_checkpoints("int8")
+    a = m(xs[0])
+    m.set_train_checkpoints(None)
+    b = m(xs[1])                                               # keeps no checkpoint; its tensors make room for a's
+    a.sum().backward()
+    with pytest.raises(RuntimeError, match="newer"):
+        b.sum().backward()
+    m.set_train_checkpoints("e4m3")
+    c = m(xs[0])
+    with torch.no_grad():
+        next(m.parameters()).mul_(1.0)
+    with pytest.raises(RuntimeError, match="in-place change"):
+        c.sum().backward()
