@@ -623,10 +623,15 @@ __global__ __launch_bounds__(T) void norm_planar_bwd_kernel(NormArgs a) {
   }
 }
 
-// Blocks of a persistent launch on 256 CUs: 2048 threads each (all their waves) for the forward, 1024 for the backward, whose registers hold the
-// next token as well and whose blocks leave a slab of weight gradients each (32x256x88x88 bf16: 94.0 against 96.5 us, 32x256x56x56
-// float 62.6 against 67.2 us with the sums of the slabs)
-static int64_t norm_blocks(int threads, bool bwd) { return 256 * (int64_t)std::max((bwd ? 1024 : 2048) / threads, 1); }
+// Blocks of a persistent launch on 256 CUs, as waves per SIMD: about what the registers of the form let a CU hold, so that the last
+// blocks do not run alone, and in the backward, whose blocks leave a slab of weight gradients each, no more than keep the loads in
+// flight (with the next token's loads ahead of the sums, two waves are enough where a lane holds much).  Measured, us (backward with
+// the sum of the slabs):
+//   rows of one piece: forward 8 / 6 / 4 waves 19.2 / 17.7 / 18.4 (65536 x 256 bf16, checkpoint); backward 4 / 3 / 2 waves 58.3 / 56.7 / 60.3
+//     (200704 x 128 float);
+//   rows of two: forward 18.3 / 16.8 / 16.6 (16384 x 1024 bf16); backward 29.5 / 26.6 / 25.8, at 16384 x 4096 107 / 91 / 92;
+//   planar: forward 43.6 / 44.9 / 46.2 (32x256x88x88 bf16); backward 95.9 / 94.1 / 94.2, at 64x40x112x112 bf16 70.7 / 71.4 / 56.3.
+static int64_t norm_blocks(int threads, int waves) { return 256 * (int64_t)std::max(256 * waves / threads, 1); }
 
 // The register forms: which one takes a case, what its grid is.  slabs = 0: none.
 struct NormPlan { int G, NV; int T, PX, NC; int64_t slabs, tiles, items; };
@@ -639,7 +644,7 @@ static NormPlan norm_plan(int rows, int a16, bool bwd, int64_t outer, int64_t C,
     p.NV = C <= (int64_t)p.G * 8 ? 1 : 2;
     p.T = std::max(p.G, CSN_BLOCK);
     const int r = p.T / p.G;
-    p.slabs = std::min(norm_blocks(p.T, bwd), (outer + r - 1) / r);
+    p.slabs = std::min(norm_blocks(p.T, p.NV == 1 ? (bwd ? 3 : 6) : (bwd ? 2 : 4)), (outer + r - 1) / r);
     return p;
   }
   if (C > 2048 || inner < NORM_PE) return p;
@@ -662,7 +667,7 @@ static NormPlan norm_plan(int rows, int a16, bool bwd, int64_t outer, int64_t C,
   p.items = outer * p.tiles;
   // 32-bit byte offsets of a lane and 32-bit item counts
   if (inner > lim || p.items > lim || cg * std::max(inner, std::max(x_sc, dy_sc)) + inner + tile > lim) { p.slabs = 0; return p; }
-  p.slabs = std::min(norm_blocks(p.T, bwd), p.items);
+  p.slabs = std::min(norm_blocks(p.T, bwd ? 2 : 8), p.items);
   return p;
 }
 
