@@ -406,8 +406,10 @@ __device__ __forceinline__ void norm_load(VecIo<AT, E>& v, const AT* base, unsig
   v.zero();
   if (n > 0) v.load(norm_at(base, bytes));
 }
+// (Four waves per SIMD: a float form with a checkpoint gives up ten registers for a second block of 512 threads on the CU, 16x512x44x44
+// 35.2 -> 31.9 us.)
 template <typename AT, int T, int PX, int NC, int CK>
-__global__ __launch_bounds__(T) void norm_planar_fwd_kernel(NormArgs a) {
+__global__ __launch_bounds__(T, 4) void norm_planar_fwd_kernel(NormArgs a) {
   constexpr int E = NORM_PE, CG = T / PX, TP = PX * E;
   CSN_DYN_SMEM(float, sm);
   const int px = threadIdx.x % PX, cg = threadIdx.x / PX, C = (int)a.C, P = (int)a.inner;
@@ -650,16 +652,17 @@ static NormPlan norm_plan(int rows, int a16, bool bwd, int64_t outer, int64_t C,
   if (C > 2048 || inner < NORM_PE) return p;
   // The forward does best with the most channels per lane that fit its registers and 16 lanes (128 / 256 bytes of a channel) across the
   // pixels: 16 channels 46 us, 8 channels 52 us (32x256x88x88 bf16), 36 against 50 us (16x512x44x44 float with a checkpoint).  The backward
-  // holds two tensors, the next tile of both and two sums per channel: 8 channels (4 in float and in blocks of 1024 threads, whose
-  // registers are half as many) 94 us, 16 channels 120 us.  Wider tokens than that narrow the tile.
+  // holds two tensors, the next tile of both and two sums per channel: 8 channels 94 us, 16 channels 120 us (32x256x88x88 bf16); 4 channels in
+  // blocks of 1024 threads, whose registers are half as many, lose in float (16x1024x32x32 80 against 63 us, 16x2048x28x28 171 against
+  // 145) and are as good in bf16 (58 against 60, 159 against 159).  Wider tokens than that narrow the tile.
   if (!bwd) {
     p.T = C <= 64 ? 128 : C <= 128 ? 128 : C <= 256 ? 256 : C <= 512 ? 512 : 1024;
     p.PX = C <= 1024 ? 16 : 8;
     p.NC = C <= 64 ? 8 : 16;
   } else {
-    p.T = C <= 64 ? 128 : C <= 128 ? 256 : C <= 256 ? 512 : 1024;
+    p.T = C <= 64 ? 128 : C <= 128 ? 256 : C <= 256 && !a16 ? 256 : 512;
     p.PX = C <= 128 ? 16 : C <= 256 ? (a16 ? 16 : 8) : C <= 512 ? 8 : C <= 1024 ? 4 : 2;
-    p.NC = C <= 128 || (C <= 256 && a16) ? 8 : 4;
+    p.NC = 8;
   }
   const int cg = p.T / p.PX;
   const int64_t tile = (int64_t)p.PX * NORM_PE, lim = (int64_t)1 << 29;
@@ -713,10 +716,10 @@ static int norm_planar_run(const NormArgs& a, const NormPlan& p, bool bwd, void*
     return p.PX == 16 ? norm_planar_fwd<AT, 1024, 16, 16, CK>(a, stream) : norm_planar_fwd<AT, 1024, 8, 16, CK>(a, stream);
   }
   if (p.T == 128) return norm_planar_bwd<AT, 128, 16, 8, CK>(a, stream);
-  if (p.T == 256) return norm_planar_bwd<AT, 256, 16, 8, CK>(a, stream);
-  if (p.T == 512) return norm_planar_bwd<AT, 512, sizeof(AT) == 2 ? 16 : 8, sizeof(AT) == 2 ? 8 : 4, CK>(a, stream);
-  if (p.PX == 8) return norm_planar_bwd<AT, 1024, 8, 4, CK>(a, stream);
-  return p.PX == 4 ? norm_planar_bwd<AT, 1024, 4, 4, CK>(a, stream) : norm_planar_bwd<AT, 1024, 2, 4, CK>(a, stream);
+  if (p.T == 256) return p.PX == 16 ? norm_planar_bwd<AT, 256, 16, 8, CK>(a, stream) : norm_planar_bwd<AT, 256, 8, 8, CK>(a, stream);
+  if (p.PX == 16) return norm_planar_bwd<AT, 512, 16, 8, CK>(a, stream);
+  if (p.PX == 8) return norm_planar_bwd<AT, 512, 8, 8, CK>(a, stream);
+  return p.PX == 4 ? norm_planar_bwd<AT, 512, 4, 8, CK>(a, stream) : norm_planar_bwd<AT, 512, 2, 8, CK>(a, stream);
 }
 template <int CK>
 static int norm_fast(const NormArgs& a, const NormPlan& p, int rows, int a16, bool bwd, void* stream) {
