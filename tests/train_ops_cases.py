@@ -224,7 +224,8 @@ def check_product(lib, dy, x, fmt, dim):
 # inside a block and a vector
 NORM_SHAPES = [((1, 1), -1), ((1, 2048), -1), ((7, 8), -1), ((5, 33), -1), ((130, 64), -1), ((3, 331), -1), ((2, 9, 80), -1), ((2, 5000), -1),
                ((1, 20000), -1), ((70, 1000), -1), ((1, 1, 1, 1), 1), ((2, 79, 5, 7), 1), ((1, 40, 28, 28), 1), ((3, 20, 1, 1), 1),
-               ((2, 8, 33), 1), ((1, 300, 6, 6), 1), ((2, 64, 16, 16), 1), ((1, 2, 100, 3), 1), ((1, 1100, 4, 8), 1), ((1, 64, 40, 40), 1), ((1, 3000, 5, 7), 1), ((1, 5000, 1, 3), 1), ((1, 33000), -1)]
+               ((2, 8, 33), 1), ((1, 300, 6, 6), 1), ((2, 64, 16, 16), 1), ((1, 2, 100, 3), 1), ((1, 1100, 4, 8), 1), ((1, 64, 40, 40), 1), ((1, 3000, 5, 7), 1), ((1, 5000, 1, 3), 1), ((1, 33000), -1),
+               ((1, 150, 6, 6), 1), ((1, 600, 5, 5), 1)]
 PACK_SHAPES = [((1,), -1), ((3, 31), -1), ((2, 32), -1), ((5, 33), -1), ((4, 64), -1), ((3, 7, 100), -1), ((2, 3, 5, 9), 2), ((1, 4, 8, 8), 2),
                ((2, 2, 1, 1), 2), ((3, 40, 14, 14), 2)]
 # (outer dims of x, cin, cout, dim)
@@ -504,9 +505,10 @@ def check_plan_checkpoint(lib, device, manifest, act_dtype, fmt, B=2, size=32):
     m = _net(lib, device, manifest, act_dtype, B)
     f = {"int8": N.Q8_INT8, "e4m3": N.Q8_E4M3}[fmt]
     x = torch.from_numpy(I.randn_batch(31, B, size, size)).to(device)
+    eng = m.engine_for(x, train=True)
+    eng.workspace.fill_(255)                                   # NaN in every type: what the forward does not write is told apart
     y, _ = m._train_forward_raw(x)
     dy = gradient(tuple(y.shape), torch.float32, 1, device)
-    eng = m.engine_for(x, train=True)
     acts = [i for i in range(1, eng.n_acts)]
     before = {}
     for i in acts:
@@ -523,7 +525,7 @@ def check_plan_checkpoint(lib, device, manifest, act_dtype, fmt, B=2, size=32):
     for (i, what), t in before.items():
         q = T.q8_pack(m._lib or N.load(), t, fmt, start_dim=2)
         v, now = T.q8_unpack(m._lib or N.load(), q), eng.train_probe(i, what)
-        if torch.equal(now, t) and not torch.equal(v, t):
+        if bool(torch.isnan(t).all()):
             assert what == "act"                              # (an activation that its consumer forms on load is not stored)
             continue
         changed += 1
