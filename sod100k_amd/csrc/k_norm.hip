@@ -4,6 +4,16 @@
 //     g = dy w,  c1 = sum_c g / C,  c2 = sum_c g xh / C,  dx = rstd (g - c1 - xh c2),  dw = sum_t dy xh,  db = sum_t dy
 //
 // with xh = (x - mean) rstd; in the backward x may be the 8-bit checkpoint that the forward left (q8_core.h).
+//
+// Bound by bytes: forward x and y, backward x, dy and dx, each once, at the 6.2 TB/s of a large copy.  A token's channels therefore stay in
+// registers over the passes that the formulas make (sum, sum of squares, output; the two sums of the backward, output), which are
+// lane exchanges and one trip through LDS.  Kernel times against that floor, us (cold caches):
+//   25088 x 512 float         forward 22.2 of 16.6   backward 29.0 of 24.8, sum of the slabs 3.9
+//   32x256x88x88 bf16         forward 48.8 of 40.9   backward 96   of 61.3, sum of the slabs 4.6
+//   16384 x 1024 bf16, int8 checkpoint    forward 22.3 of 13.6   backward 26.0 of 13.6, sum of the slabs 4.0
+//   16x512x44x44 float, e4m3 checkpoint   forward 36   of 23.1   backward 47   of 23.1, sum of the slabs 4.8
+// The forward of maps waits for its loads between blocks (no room for the next tile beside 16 channels); the backward has the next tile
+// in flight, and what is left is the arithmetic and the exchanges between a tile's loads and its stores, two waves per SIMD.
 #include "csn_reduce.h"
 #include "q8_core.h"
 #include "slab_sum.h"

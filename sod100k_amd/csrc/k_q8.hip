@@ -1,6 +1,8 @@
 // k_q8.hip -- 8-bit checkpoints of activations: pack and unpack (format and decisions: q8_core.h).
 //
-// Both are streams: pack reads 4 or 2 bytes an element and writes 1 + 1/32, unpack the reverse.
+// Both are streams: pack reads 4 or 2 bytes an element and writes 1 + 1/32, unpack the reverse.  64x40x224x224 bf16, int8: pack
+// 78 us (5.0 TB/s; with the tensor in the cache of the device 69), unpack 66 us (5.9 TB/s) where a plain copy moves 6.2 TB/s; small tensors
+// (40x56x56) 2.8 us each, what a launch costs.
 //
 // A lane takes a piece of 16 (bfloat16) or 8 (float) consecutive elements, so that codes move 16 or 8 bytes at a time; the two or four lanes of
 // a block exchange its maximum.  Pieces are counted through rows of `per_row` pieces each, a row's last block being short; rows
