@@ -62,6 +62,7 @@ struct NormArgs {
   // set by the launcher
   int32_t slabs;            // blocks of the register forms
   int32_t tiles, items;     // planar: pixel tiles of an image, (image, tile) items
+  int32_t runs;             // planar: items by XCD
 };
 int csn_launch_norm_fwd(const NormArgs& a, int rows, int a16, int fmt, void* stream);
 int csn_launch_norm_bwd(const NormArgs& a, int rows, int a16, int fmt, void* stream);

@@ -89,11 +89,21 @@ def _view(x: torch.Tensor, rows: bool) -> Tuple[torch.Tensor, int, int]:
     if x.is_contiguous():
         ch = x.shape[-1] if rows else x.shape[1]
         return (x, ch, 0) if rows else (x, x.numel() // x.shape[0], x.numel() // (x.shape[0] * ch))
-    v = x.reshape(-1, x.shape[-1]) if rows else x.flatten(2)
-    if v.shape[-1] > 1 and v.stride(-1) != 1:
-        v = v.contiguous()
-    so = v.stride(0) if v.shape[0] > 1 else 0
-    return v, so, (0 if rows or v.shape[1] <= 1 else v.stride(1))
+    shape, stride = x.shape, x.stride()
+    end, n = (len(shape) - 1, -1) if rows else (len(shape), 1)     # the axes [0, end) / [2, end) have to lie as one, n apart (-1: any)
+    if rows and shape[-1] > 1 and stride[-1] != 1:
+        return x.contiguous(), shape[-1], 0
+    so = 0
+    for d in range(end - 1, -1 if rows else 1, -1):
+        if shape[d] > 1:
+            if n == -1:
+                n = so = stride[d]
+            elif stride[d] != n:
+                return _view(x.contiguous(), rows)
+            n *= shape[d]
+    if rows:
+        return x, so, 0
+    return x, stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else 0
 
 
 def _blocks(cols: int) -> int:
