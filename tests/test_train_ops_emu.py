@@ -140,3 +140,25 @@ def test_plan_checkpoint_refusals(lib, x2_manifest):
     assert lib.csn_plan_checkpoint_bytes(ev.plan) == 0
     with pytest.raises(ValueError):
         m.set_train_checkpoints("fp4")
+
+
+def test_views_of_slices():
+    """Every slice, permutation and broadcast that is read as it lies, or copied, has the elements of the tensor in its order."""
+    from sod100k_amd.train_ops import _view
+    base = torch.arange(4 * 6 * 3 * 5).reshape(4, 6, 3, 5)
+    cuts = (slice(None), slice(1, None), slice(0, 1), slice(None, None, 2))
+    as_it_lies = 0
+    for perm in ((0, 1, 2, 3), (1, 0, 2, 3), (0, 2, 3, 1), (3, 2, 1, 0)):
+        for cut in ((a, b, c, d) for a in cuts for b in cuts for c in cuts for d in cuts):
+            x = base.permute(perm)[cut]
+            for t in (x, x[:, :, :1].expand(-1, -1, 3, -1), x[:1].expand(2, -1, -1, -1), x[0], x[0, 0]):
+                for rows in (True, False) if t.dim() > 2 else (True,):
+                    v, so, sc = _view(t, rows)
+                    want = t.reshape(-1, t.shape[-1]) if rows else t.flatten(2)
+                    got = torch.as_strided(v, want.shape, (so, 1) if rows else (so, sc, 1), v.storage_offset())
+                    assert torch.equal(got, want)
+                    as_it_lies += v.data_ptr() == t.data_ptr()
+    assert as_it_lies > 1000
+    x = torch.zeros(4, 10, 6, 7)
+    for t, rows in ((x[:, 2:9], False), (x[1:], False), (x.reshape(-1, 7)[:, 1:5], True), (x[..., 2:], True)):
+        assert _view(t, rows)[0].data_ptr() == t.data_ptr()      # slices of channels and images are not copied
