@@ -379,19 +379,6 @@ __device__ __forceinline__ csn_f4 csn_mfma_16x16x32_bf16(csn_u4 a, csn_u4 b, csn
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), acc, 0, 0, 0);
 #endif
 }
-// ds_read_b64_tr_b16: four 16-bit elements per lane from LDS, transposed within 16 lanes: result r of lane i is element i % 4 of lane
-// 4 r + i / 4 of the 16.  Lanes 4 r .. 4 r + 3 point at 16 consecutive elements of row r; lane i ends with column i of the four rows.
-__device__ __forceinline__ uint2 csn_lds_read_tr16(const unsigned char* p) {
-  uint2 r;
-#ifdef CSN_EMU_LANES
-  csn_emu::lanes_read_tr16_b64(p, &r);
-#else
-  typedef short s4 __attribute__((ext_vector_type(4)));
-  const s4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(const_cast<unsigned char*>(p)));
-  r = __builtin_bit_cast(uint2, v);
-#endif
-  return r;
-}
 #endif  // !CSN_EMU_SEQ
 // v_alignbit_b32: the low dword of ({hi, lo} >> sh)
 __device__ __forceinline__ unsigned csn_alignbit(unsigned hi, unsigned lo, unsigned sh) {

@@ -1,9 +1,25 @@
 // csn_train_ops.inl -- C entry points of the training operators beside the plan (include/csnet_hip.h): argument checks, workspaces.
 // Included by csn_plan.hip.
 
+#ifdef CSN_CPU_EMU
+// The emulator may be built from the plan's units alone: the launchers of k_q8.hip, k_norm.hip and k_q8_wgrad.hip are then null and the entry
+// points below refuse every call.  (The product library names them firmly: a missing unit does not load.)
+#define WEAK_LAUNCHER(f) extern decltype(f) f __attribute__((weak))
+WEAK_LAUNCHER(csn_launch_q8_pack); WEAK_LAUNCHER(csn_launch_q8_unpack); WEAK_LAUNCHER(csn_launch_q8_segments); WEAK_LAUNCHER(csn_launch_copy_segments);
+WEAK_LAUNCHER(csn_launch_norm_fwd); WEAK_LAUNCHER(csn_launch_norm_bwd); WEAK_LAUNCHER(csn_norm_partial_floats);
+WEAK_LAUNCHER(csn_launch_q8_wgrad); WEAK_LAUNCHER(csn_q8_wgrad_partial_floats);
+#undef WEAK_LAUNCHER
+#endif
+
 namespace {
 
+#ifdef CSN_CPU_EMU
+inline bool train_ops_linked() { return csn_launch_q8_pack && csn_launch_norm_fwd && csn_launch_q8_wgrad; }
+#else
+inline bool train_ops_linked() { return true; }
+#endif
 #define REFUSE(why) do { g_hip_err = (why); return CSN_E_INVALID; } while (0)
+#define REFUSE_UNLINKED() do { if (!train_ops_linked()) { g_hip_err = "built without the training operators' kernels"; return CSN_E_UNSUPPORTED; } } while (0)
 
 // element counts and byte offsets of all tensors stay far inside 63 bits, block counts inside a grid
 const int64_t kMaxElems = (int64_t)1 << 46;
@@ -19,6 +35,7 @@ inline bool layout_ok(int32_t l) { return l == CSN_LAYOUT_PLANAR || l == CSN_LAY
 inline bool stride_ok(int64_t s, int64_t n) { return s >= 0 && mul_ok(n, s); }
 
 int norm_check(const csn_norm_desc* d) {
+  REFUSE_UNLINKED();
   if (!d) REFUSE("layer norm: null descriptor");
   if (!layout_ok(d->layout) || !dtype_ok(d->dtype)) REFUSE("layer norm: unknown layout or dtype");
   if (d->outer < 0 || d->inner < 0 || d->channels < 1 || d->channels > kMaxChannels)
@@ -29,6 +46,7 @@ int norm_check(const csn_norm_desc* d) {
   return CSN_OK;
 }
 int product_check(const csn_product_desc* d) {
+  REFUSE_UNLINKED();
   if (!d) REFUSE("product gradient: null descriptor");
   if (!layout_ok(d->layout) || !dtype_ok(d->dtype) || !format_ok(d->format)) REFUSE("product gradient: unknown layout, dtype or format");
   if (d->outer < 0 || d->inner < 0 || d->cin < 1 || d->cout < 1 || d->cin > kMaxChannels || d->cout > kMaxChannels || d->cin * d->cout > ((int64_t)1 << 40))
@@ -107,6 +125,7 @@ extern "C" {
 size_t csn_plan_checkpoint_bytes(const csn_plan* P) { return P && P->train ? (size_t)plan_saved_bytes(P) : 0; }
 
 int csn_plan_checkpoint_save(csn_plan* P, const void* workspace, int32_t format, void* checkpoint, size_t checkpoint_bytes, void* stream) {
+  REFUSE_UNLINKED();
   if (!P || !workspace || !checkpoint || ((uintptr_t)checkpoint & 255u) || !format_ok(format)) REFUSE("plan checkpoint: null or misaligned (256 bytes) buffer, unknown format");
   if (!P->train || !P->bn_tables_train) { g_hip_err = "plan checkpoint: no train-mode forward of a training plan to save"; return CSN_E_STATE; }
   if (checkpoint_bytes < (size_t)plan_saved_bytes(P)) REFUSE("plan checkpoint: buffer smaller than csn_plan_checkpoint_bytes");
@@ -114,6 +133,7 @@ int csn_plan_checkpoint_save(csn_plan* P, const void* workspace, int32_t format,
 }
 
 int csn_plan_checkpoint_restore(csn_plan* P, void* workspace, int32_t format, const void* checkpoint, size_t checkpoint_bytes, void* stream) {
+  REFUSE_UNLINKED();
   if (!P || !workspace || !checkpoint || ((uintptr_t)checkpoint & 255u) || !format_ok(format)) REFUSE("plan checkpoint: null or misaligned (256 bytes) buffer, unknown format");
   if (!P->train || !P->bn_tables_train) { g_hip_err = "plan checkpoint: a training plan that has run a forward is needed"; return CSN_E_STATE; }
   if (checkpoint_bytes < (size_t)plan_saved_bytes(P)) REFUSE("plan checkpoint: buffer smaller than csn_plan_checkpoint_bytes");
@@ -122,6 +142,7 @@ int csn_plan_checkpoint_restore(csn_plan* P, void* workspace, int32_t format, co
 
 int csn_q8_pack(const void* x, int32_t dtype, int64_t outer, int64_t rows, int64_t cols, int64_t outer_stride, int64_t row_stride,
                 int32_t format, uint8_t* codes, uint8_t* exponents, void* stream) {
+  REFUSE_UNLINKED();
   if (!dtype_ok(dtype) || !format_ok(format)) REFUSE("q8 pack: unknown dtype or format");
   if (outer < 0 || rows < 0 || cols < 0 || !mul_ok(outer, rows) || !mul_ok(outer * rows, cols)) REFUSE("q8 pack: negative or too large sizes");
   if (!stride_ok(outer_stride, outer) || !stride_ok(row_stride, rows)) REFUSE("q8 pack: negative or too large strides");
@@ -136,6 +157,7 @@ int csn_q8_pack(const void* x, int32_t dtype, int64_t outer, int64_t rows, int64
 
 int csn_q8_unpack(const uint8_t* codes, const uint8_t* exponents, int32_t format, int64_t rows, int64_t cols, void* y, int32_t dtype,
                   void* stream) {
+  REFUSE_UNLINKED();
   if (!dtype_ok(dtype) || !format_ok(format)) REFUSE("q8 unpack: unknown dtype or format");
   if (rows < 0 || cols < 0 || !mul_ok(rows, cols)) REFUSE("q8 unpack: negative or too large sizes");
   if (rows == 0 || cols == 0) return CSN_OK;

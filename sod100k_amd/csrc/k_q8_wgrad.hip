@@ -46,6 +46,23 @@ __device__ __forceinline__ csn_u4 wg_u4(unsigned a, unsigned b, unsigned c, unsi
   r.x = a; r.y = b; r.z = c; r.w = d;
   return r;
 }
+// ds_read_b64_tr_b16: four 16-bit elements per lane from LDS, transposed within 16 lanes: result r of lane i is element i % 4 of lane
+// 4 r + i / 4 of the 16.  Lanes 4 r .. 4 r + 3 point at 16 consecutive elements of row r; lane i ends with column i of the four rows.
+__device__ __forceinline__ uint2 wg_read_tr16(const unsigned char* p) {
+  uint2 r;
+#ifdef CSN_EMU_LANES
+  const unsigned lane = threadIdx.x & 63, i = lane & 15;
+  const csn_emu::Xchg x = csn_emu::wave_xchg(11, nullptr, p, 8, true);
+  unsigned short v[4];
+  for (unsigned k = 0; k < 4; ++k) __builtin_memcpy(&v[k], x.tab + 64 * ((lane & ~15u) + 4 * k + (i >> 2)) + 2 * (i & 3), 2);
+  __builtin_memcpy(&r, v, 8);
+#else
+  typedef short s4 __attribute__((ext_vector_type(4)));
+  const s4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(const_cast<unsigned char*>(p)));
+  r = __builtin_bit_cast(uint2, v);
+#endif
+  return r;
+}
 // {the high halves of a and b}: two bfloat16 by truncation
 __device__ __forceinline__ unsigned wg_hi2(float a, float b) {
 #ifdef CSN_CPU_EMU
@@ -315,7 +332,7 @@ __global__ __launch_bounds__((WgShape<AT, ROWS, TM, TN>::T)) void q8_wgrad_kerne
     }
   }
   auto read8 = [&](const unsigned char* p, const unsigned char* q) {
-    const uint2 lo = csn_lds_read_tr16(p), hi = csn_lds_read_tr16(q);
+    const uint2 lo = wg_read_tr16(p), hi = wg_read_tr16(q);
     return wg_u4(lo.x, lo.y, hi.x, hi.y);
   };
   auto multiply = [&](const unsigned char* buf) {

@@ -103,7 +103,6 @@ void lanes_mfma_f32_16x16x32_bf16(const void* a8, const void* b8, float* d4);
 unsigned lanes_dpp_wave_shr1(unsigned v);   // lane i <- lane i - 1 (row_shr across the wave, bound_ctrl: 0 where there is no source)
 unsigned lanes_dpp_wave_shl1(unsigned v);   // lane i <- lane i + 1
 unsigned lanes_readfirstlane(unsigned v);
-void lanes_read_tr16_b64(const void* p8, void* out8);   // ds_read_b64_tr_b16: see below
 unsigned long long lanes_shfl_xor64(unsigned long long v, int x);   // the 64-bit value of lane (lane ^ x): __shfl_xor(v, x, 64)
 void lanes_wave_sync();
 #endif
@@ -390,15 +389,6 @@ __attribute__((noinline)) unsigned long long lanes_shfl_xor64(unsigned long long
   unsigned long long r; std::memcpy(&r, x.tab + 64 * srcl, 8);
   return r;
 }
-// ds_read_b64_tr_b16: every lane reads four 16-bit elements at its own address; within 16 lanes, result r (0 .. 3) of lane i is element
-// i % 4 of lane 4 r + i / 4 -- the 16 lanes' data taken as four rows of 16 elements, lane i gets column i
-__attribute__((noinline)) void lanes_read_tr16_b64(const void* p8, void* out8) {
-  const unsigned lane = cur_thread() & 63, base = lane & ~15u, i = lane & 15;
-  const Xchg x = wave_xchg(11, __builtin_return_address(0), p8, 8, true);
-  unsigned short r[4];
-  for (unsigned k = 0; k < 4; ++k) std::memcpy(&r[k], x.tab + 64 * (base + 4 * k + (i >> 2)) + 2 * (i & 3), 2);
-  std::memcpy(out8, r, 8);
-}
 __attribute__((noinline)) void lanes_wave_sync() { (void)wave_xchg(9, __builtin_return_address(0), nullptr, 0, false); }
 #endif
 
@@ -519,7 +509,7 @@ void launch_named(const char* name, dim3 grid, dim3 block, size_t smem_bytes, co
 }  // namespace csn_emu
 #ifdef CSN_EMU_LANES
 // tests: the number of cross-lane instructions executed so far (kind: 1 mfma 4x4x1, 2 4x4x4 bf16, 3 16x16x4, 4 32x32x16 bf16,
-// 5 16x16x32 bf16, 6 / 7 DPP wave_shr / wave_shl, 8 readfirstlane, 9 wave sync, 10 shuffle-xor, 11 transposing LDS read); proof that the lane-exact paths ran
+// 5 16x16x32 bf16, 6 / 7 DPP wave_shr / wave_shl, 8 readfirstlane, 9 wave sync, 10 shuffle-xor); proof that the lane-exact paths ran
 extern "C" unsigned long long csn_emu_lane_ops(int kind) { return csn_emu::g_lane_ops[kind & 15]; }
 #endif
 #endif  // CSN_EMU_IMPL
