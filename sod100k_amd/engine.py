@@ -107,6 +107,7 @@ class Engine:
         self.plan = plan
         self.train = bool(train)
         self.input_grad = bool(train) and bool(input_grad)
+        self.train_bf16 = bool(train) and bool(train_bf16)
         if self.train:      # z / gradient / scratch buffers + backward weight images (before the workspace query)
             if train_bf16:  # BEFORE the training buffers are laid out: every activation-typed region gets 2-byte elements
                 self.set_option(N.OPT_TRAIN_BF16, 1)

@@ -517,7 +517,8 @@ class CSNet(nn.Module):
         activations, so with "int8" or "e4m3" the next forward first puts the previous one's saved tensors, if its graph is
         still waiting for its backward, into an 8-bit checkpoint (csn_plan_checkpoint_save; a quarter / half of the fp32 / bf16
         tensors).  The last forward's own backward is exact, an earlier one's has the gradients of the checkpoint's values; a step
-        with one forward costs nothing.  None (default): a backward after a newer forward raises."""
+        with one forward costs nothing.  Parameters, and with float32 activations the image batch, stay as they are while a forward
+        waits: a change in place raises in its backward.  None (default): a backward after a newer forward raises."""
         if format not in (None, "int8", "e4m3"):
             raise ValueError("train checkpoints must be 'int8', 'e4m3' or None")
         self._train_checkpoints = format
@@ -665,6 +666,9 @@ class _CSNetTrainFn(torch.autograd.Function):
         eng, arena = s.engine, model._arena
         if s.versions != _versions(model):
             raise RuntimeError("CSNet backward after an in-place change of the parameters: its gradients are those of the forward's")
+        if s.x_version is not None and s.x_version != ctx.x._version:
+            raise RuntimeError("CSNet backward after an in-place change of the image batch: its gradients are those of the forward's "
+                               "(give every forward that waits a batch of its own)")
         if eng.waiting is not None and eng.waiting() is s:
             pass
         elif s.checkpoint is not None:
@@ -694,6 +698,8 @@ class _SavedForward:
     def __init__(self, model, x, format):
         self.engine, self.format, self.flop_tab, self.checkpoint = model.engine_for(x, train=True), format, model._flop_tab, None
         self.versions = _versions(model)
+        # float32 steps read the image batch again in the backward (bfloat16 ones keep a copy of their own, which is saved)
+        self.x_version = None if self.engine.train_bf16 or x.is_inference() else x._version
         self.engine.waiting = weakref.ref(self)
 
 

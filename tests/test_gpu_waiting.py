@@ -1,0 +1,21 @@
+"""Forwards that wait for their backward (CSNet.set_train_checkpoints) on the GPU."""
+import pytest
+import torch
+
+import waiting_cases as W
+from sod100k_amd import _native as N
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not torch.cuda.is_available():
+        pytest.fail("the GPU suite needs a ROCm device")
+    return N.load()
+
+
+@pytest.mark.parametrize("act_dtype", ["fp32", "bf16"])
+def test_gpu_refilled_batch(lib, x2_manifest, act_dtype):
+    W.check_refilled_batch(lib, DEV, x2_manifest, act_dtype)
