@@ -5,6 +5,7 @@ PyTorch is used here for device memory and streams only (``tensor.data_ptr()``,
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 from typing import Dict, List, Optional, Sequence, Tuple
@@ -128,6 +129,7 @@ class Engine:
         self.n_acts = len(acts)
         nbytes = int(lib.csn_plan_workspace_bytes(plan))
         self.workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+        self._used, self._used_on = None, None      # of a training plan: event behind its last launch and the stream of that launch
 
     def __del__(self):
         plan = getattr(self, "plan", None)
@@ -143,10 +145,32 @@ class Engine:
             return torch.cuda.current_stream(self.device).cuda_stream
         return 0
 
+    @contextlib.contextmanager
+    def _in_turn(self):
+        """Around the launches of a training plan: a forward, the checkpoints and the backwards share one workspace and one set of
+        packed tables, and autograd runs every backward on its forward's stream.  Work on another stream than the last one's waits
+        for it there.  (Not inside a caller's stream capture: its order is the caller's.)"""
+        if not self.train or self.device.type != "cuda" or torch.cuda.is_current_stream_capturing():
+            yield
+            return
+        stream = torch.cuda.current_stream(self.device)
+        if self._used is None:
+            self._used = torch.cuda.Event()
+        elif self._used_on != stream.cuda_stream:
+            stream.wait_event(self._used)
+            if self.workspace.is_cuda:              # (allocated on the stream of the plan's first call)
+                self.workspace.record_stream(stream)
+        try:
+            yield
+        finally:                                    # (also where a call failed half way)
+            self._used.record(stream)
+            self._used_on = stream.cuda_stream
+
     def refresh(self, arena: torch.Tensor) -> None:
         assert arena.dtype == torch.float32 and arena.is_contiguous() and arena.device == self.workspace.device
-        N.check(self.lib, self.lib.csn_plan_refresh_params(self.plan, arena.data_ptr(), arena.numel(),
-                                                           self._stream()), "csn_plan_refresh_params")
+        with self._in_turn():
+            N.check(self.lib, self.lib.csn_plan_refresh_params(self.plan, arena.data_ptr(), arena.numel(),
+                                                               self._stream()), "csn_plan_refresh_params")
 
     def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         assert x.dtype == torch.float32 and x.shape[0] == self.B and tuple(x.shape[2:]) == (self.H, self.W), \
@@ -165,9 +189,10 @@ class Engine:
         x = x.contiguous()
         y = out if out is not None else torch.empty((self.B, 1, self.H, self.W), dtype=torch.float32, device=x.device)
         fw = (C.c_float * (self.n_units * N.MAX_BRANCH))(*[float(v) for v in flop_w])
-        N.check(self.lib, self.lib.csn_forward_train(self.plan, x.data_ptr(), y.data_ptr(), self.workspace.data_ptr(),
-                                                     arena.data_ptr(), arena.numel(), fw, penalty.data_ptr(),
-                                                     self._stream()), "csn_forward_train")
+        with self._in_turn():
+            N.check(self.lib, self.lib.csn_forward_train(self.plan, x.data_ptr(), y.data_ptr(), self.workspace.data_ptr(),
+                                                         arena.data_ptr(), arena.numel(), fw, penalty.data_ptr(),
+                                                         self._stream()), "csn_forward_train")
         return y
 
     def backward(self, x: torch.Tensor, dy: torch.Tensor, arena: torch.Tensor, grad: torch.Tensor, flop_w,
@@ -177,9 +202,10 @@ class Engine:
         assert dy.dtype == torch.float32 and dy.is_contiguous() and dy.numel() == self.B * self.H * self.W
         assert grad.dtype == torch.float32 and grad.is_contiguous() and grad.device == arena.device
         fw = (C.c_float * (self.n_units * N.MAX_BRANCH))(*[float(v) for v in flop_w])
-        N.check(self.lib, self.lib.csn_backward(self.plan, x.data_ptr(), dy.data_ptr(), self.workspace.data_ptr(),
-                                                arena.data_ptr(), grad.data_ptr(), grad.numel(), fw,
-                                                float(pen_scale), self._stream()), "csn_backward")
+        with self._in_turn():
+            N.check(self.lib, self.lib.csn_backward(self.plan, x.data_ptr(), dy.data_ptr(), self.workspace.data_ptr(),
+                                                    arena.data_ptr(), grad.data_ptr(), grad.numel(), fw,
+                                                    float(pen_scale), self._stream()), "csn_backward")
 
     def checkpoint_save(self, format: int) -> torch.Tensor:
         """8-bit checkpoint (``_native.Q8_INT8`` / ``Q8_E4M3``) of the last ``forward_train``: what ``backward`` reads of it."""
@@ -187,8 +213,9 @@ class Engine:
         n = int(self.lib.csn_plan_checkpoint_bytes(self.plan))
         buf = torch.empty(n + 255, dtype=torch.uint8, device=self.device)
         buf = buf[-buf.data_ptr() % 256:][:n]
-        N.check(self.lib, self.lib.csn_plan_checkpoint_save(self.plan, self.workspace.data_ptr(), format, buf.data_ptr(), n,
-                                                            self._stream()), "csn_plan_checkpoint_save")
+        with self._in_turn():
+            N.check(self.lib, self.lib.csn_plan_checkpoint_save(self.plan, self.workspace.data_ptr(), format, buf.data_ptr(), n,
+                                                                self._stream()), "csn_plan_checkpoint_save")
         return buf
 
     def checkpoint_restore(self, buf: torch.Tensor, format: int) -> None:
@@ -196,8 +223,9 @@ class Engine:
         assert buf.dtype == torch.uint8 and buf.is_contiguous() and buf.device == self.workspace.device
         if buf.is_cuda:      # (allocated on the stream of the forward that displaced it)
             buf.record_stream(torch.cuda.current_stream(self.device))
-        N.check(self.lib, self.lib.csn_plan_checkpoint_restore(self.plan, self.workspace.data_ptr(), format, buf.data_ptr(),
-                                                               buf.numel(), self._stream()), "csn_plan_checkpoint_restore")
+        with self._in_turn():
+            N.check(self.lib, self.lib.csn_plan_checkpoint_restore(self.plan, self.workspace.data_ptr(), format, buf.data_ptr(),
+                                                                   buf.numel(), self._stream()), "csn_plan_checkpoint_restore")
 
     def profile(self, x: torch.Tensor, iters: int = 10):
         """Mean milliseconds per unit (HIP events on the launch stream), kernel names, algorithmic bytes."""
@@ -255,7 +283,8 @@ class Engine:
                "dz": ti.dz_offset_bytes, "grad0": ti.grad_offset_bytes[0], "grad1": ti.grad_offset_bytes[1]}[what]
         if off < 0:
             raise ValueError(f"activation {act_id} has no '{what}' buffer")
-        return self._ws_tensor(off, act_id, bf16).to(torch.float32).clone()
+        with self._in_turn():
+            return self._ws_tensor(off, act_id, bf16).to(torch.float32).clone()
 
     def n_consumers(self, act_id: int) -> int:
         ti = N.TrainActInfo()

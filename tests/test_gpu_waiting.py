@@ -19,3 +19,8 @@ def lib():
 @pytest.mark.parametrize("act_dtype", ["fp32", "bf16"])
 def test_gpu_refilled_batch(lib, x2_manifest, act_dtype):
     W.check_refilled_batch(lib, DEV, x2_manifest, act_dtype)
+
+
+@pytest.mark.parametrize("act_dtype", ["fp32", "bf16"])
+def test_gpu_two_streams(lib, x2_manifest, act_dtype):
+    W.check_two_streams(lib, DEV, x2_manifest, act_dtype, B=8, size=96, rounds=3)

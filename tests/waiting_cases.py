@@ -48,3 +48,28 @@ def check_refilled_batch(lib, device, manifest, act_dtype):
         x.zero_()
         with pytest.raises(RuntimeError, match="image batch"):
             c.backward(dy)
+
+
+def check_two_streams(lib, device, manifest, act_dtype, B, size, rounds):
+    """Forward a on one stream, forward b on another that waits for it, one backward over both: autograd runs b's node on b's stream and
+    a's on a's, with no wait between them.  The gradients are those of one stream."""
+    xs = [batch(s, device, B, size) for s in (31, 32)]
+    dy = K.gradient((B, 1, size, size), torch.float32, 1, device)
+    m = net(lib, device, manifest, act_dtype, B=B)
+    a, b = (m(x) for x in xs)
+    torch.autograd.backward([a, b], [dy, dy])
+    want = grads(m)
+    streams = [torch.cuda.Stream(device) for _ in range(2)]
+    for _ in range(rounds):
+        m = net(lib, device, manifest, act_dtype, B=B)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(streams[0]):
+            a = m(xs[0])
+        streams[1].wait_stream(streams[0])
+        with torch.cuda.stream(streams[1]):
+            b = m(xs[1])
+        for s in streams:
+            torch.cuda.current_stream().wait_stream(s)
+        torch.autograd.backward([a, b], [dy, dy])
+        torch.cuda.synchronize()
+        assert torch.equal(grads(m), want)
