@@ -87,6 +87,7 @@ def broadcast_model_(model, src: int = 0) -> None:
         return
     arena = model._ensure_arena()
     dist.broadcast(arena.flat, src=src)
+    arena.wrote()
     for name, buf in model.named_buffers():
         if name.endswith("num_batches_tracked"):
             dist.broadcast(buf, src=src)

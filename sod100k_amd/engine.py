@@ -33,7 +33,12 @@ class ParamArena:
         self.offsets: Dict[str, int] = {}
         self.flat: Optional[torch.Tensor] = None
         self.n_param_floats = 0
+        self.writes = 0            # writes into ``flat`` by raw pointer, which torch's version counters do not see (wrote())
         self.rebuild()
+
+    def wrote(self) -> None:
+        """Every writer of the parameters that goes past their tensors calls this (the fused optimizer, the broadcast of a model)."""
+        self.writes += 1
 
     def rebuild(self) -> None:
         items: List[Tuple[str, torch.Tensor, object, str, bool]] = []

@@ -517,7 +517,7 @@ class CSNet(nn.Module):
         activations, so with "int8" or "e4m3" the next forward first puts the previous one's saved tensors, if its graph is
         still waiting for its backward, into an 8-bit checkpoint (csn_plan_checkpoint_save; a quarter / half of the fp32 / bf16
         tensors).  The last forward's own backward is exact, an earlier one's has the gradients of the checkpoint's values; a step
-        with one forward costs nothing.  Parameters, and with float32 activations the image batch, stay as they are while a forward
+        with one forward pays a copy of the parameters.  Parameters, and with float32 activations the image batch, stay as they are while a forward
         waits: a change in place raises in its backward.  None (default): a backward after a newer forward raises."""
         if format not in (None, "int8", "e4m3"):
             raise ValueError("train checkpoints must be 'int8', 'e4m3' or None")
@@ -663,8 +663,8 @@ class _CSNetTrainFn(torch.autograd.Function):
         """Backward with set_train_checkpoints: of the tensors in the workspace if this forward's still lie there untouched, else of
         its checkpoint."""
         model, s = ctx.model, ctx.saved
-        eng, arena = s.engine, model._arena
-        if s.versions != _versions(model):
+        eng, arena = s.engine, s.arena
+        if model._arena is not arena or s.versions != _versions(model):
             raise RuntimeError("CSNet backward after an in-place change of the parameters: its gradients are those of the forward's")
         if s.x_version is not None and s.x_version != ctx.x._version:
             raise RuntimeError("CSNet backward after an in-place change of the image batch: its gradients are those of the forward's "
@@ -683,7 +683,7 @@ class _CSNetTrainFn(torch.autograd.Function):
         if dy is None:
             dy = torch.zeros((ctx.x.shape[0], 1) + tuple(ctx.x.shape[2:]), dtype=torch.float32, device=ctx.x.device)
         flat = torch.zeros(arena.n_param_floats, dtype=torch.float32, device=ctx.x.device)
-        eng.backward(ctx.x.contiguous(), dy.contiguous(), arena.flat, flat, s.flop_tab, float(dpen) if dpen is not None else 0.0)
+        eng.backward(ctx.x.contiguous(), dy.contiguous(), s.params, flat, s.flop_tab, float(dpen) if dpen is not None else 0.0)
         dx = eng.train_probe(0, "grad0") if ctx.input_grad else None
         model._want_input_grad = False
         grads = [flat[arena.offsets[n]:arena.offsets[n] + p.numel()].view(p.shape) if p.requires_grad else None
@@ -697,15 +697,16 @@ class _SavedForward:
 
     def __init__(self, model, x, format):
         self.engine, self.format, self.flop_tab, self.checkpoint = model.engine_for(x, train=True), format, model._flop_tab, None
-        self.versions = _versions(model)
+        # csn_backward reads the normalisations' weights: the forward's, whatever is written past the counters below (param.data)
+        self.arena, self.params, self.versions = model._arena, model._arena.flat.clone(), _versions(model)
         # float32 steps read the image batch again in the backward (bfloat16 ones keep a copy of their own, which is saved)
         self.x_version = None if self.engine.train_bf16 or x.is_inference() else x._version
         self.engine.waiting = weakref.ref(self)
 
 
 def _versions(model):
-    """What in-place changes of the parameters by torch move (a forward that waits must not see any)."""
-    return [p._version for p in model.parameters()]
+    """What in-place changes of the parameters move, torch's and the framework's own (a forward that waits must not see any)."""
+    return [model._arena.writes] + [p._version for p in model.parameters()]
 
 
 # ---- dynamic weight decay hook (csnet.py:391-410) -----------------------------------------------------------

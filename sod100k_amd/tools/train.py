@@ -106,6 +106,7 @@ class FusedTrainer:
                                                  self.v.data_ptr(), self.wd.data_ptr(), self.n, self.lr,
                                                  self.betas[0], self.betas[1], self.eps, self.steps,
                                                  self._stream(y)), "csn_adam_step")
+        model._arena.wrote()
         return self.loss.clone(), pen.clone() / bs
 
     # ---- checkpointing in torch.optim.Adam's own format (train.py:172-181 saves optimizer.state_dict()) ----

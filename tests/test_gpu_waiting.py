@@ -24,3 +24,7 @@ def test_gpu_refilled_batch(lib, x2_manifest, act_dtype):
 @pytest.mark.parametrize("act_dtype", ["fp32", "bf16"])
 def test_gpu_two_streams(lib, x2_manifest, act_dtype):
     W.check_two_streams(lib, DEV, x2_manifest, act_dtype, B=8, size=96, rounds=3)
+
+
+def test_gpu_changed_parameters(lib, x2_manifest):
+    W.check_changed_parameters(lib, DEV, x2_manifest)

@@ -77,3 +77,7 @@ def test_uses_of_the_workspace_wait_for_each_other(lib, x2_manifest, monkeypatch
         assert log == []                                      # inside a capture the order is the caller's
     finally:
         eng.device = real
+
+
+def test_emu_changed_parameters(lib, x2_manifest):
+    W.check_changed_parameters(lib, CPU, x2_manifest)

@@ -73,3 +73,43 @@ def check_two_streams(lib, device, manifest, act_dtype, B, size, rounds):
         torch.autograd.backward([a, b], [dy, dy])
         torch.cuda.synchronize()
         assert torch.equal(grads(m), want)
+
+
+def check_changed_parameters(lib, device, manifest):
+    """Parameters that something other than a torch operation on them changes while a forward waits: the fused optimizer's step and a
+    model that was moved are refused, before and after the forward was displaced; a write through ``.data``, which leaves no trace,
+    changes nothing: the gradients are those of the forward's parameters."""
+    from sod100k_amd.tools.train import FusedTrainer
+    x, other = batch(31, device), batch(32, device)
+    dy = K.gradient((1, 1, 16, 16), torch.float32, 1, device)
+    m = net(lib, device, manifest)
+    m(x).backward(dy)
+    exact = grads(m)
+    a, b = m(x), m(other)
+    a.backward(dy)
+    kept = grads(m)
+    del b
+
+    m = net(lib, device, manifest)
+    tr = FusedTrainer(m, lr=1e-2, lib=lib)
+    a = m(x)
+    tr.step(other, torch.zeros(1, 1, 16, 16, device=device))
+    with pytest.raises(RuntimeError, match="in-place change"):
+        a.backward(dy)
+    m = net(lib, device, manifest)
+    a = m(x)
+    m._apply(lambda t: t)
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="in-place change"):
+            a.backward(dy)
+        m.eval()(x)                          # (there is an arena again, another one)
+        m.train()
+    for displaced, want in ((False, exact), (True, kept)):
+        m = net(lib, device, manifest)
+        a = m(x)
+        for p in m.parameters():
+            p.data.mul_(1.5)
+        if displaced:
+            b = m(other)
+        a.backward(dy)
+        assert torch.equal(grads(m), want)
