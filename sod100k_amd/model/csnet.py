@@ -573,10 +573,7 @@ class CSNet(nn.Module):
         """(logits, fp64 device scalar penalty SUM) of one train-mode forward; keeps what csn_backward needs."""
         eng = self.engine_for(x, train=with_backward)
         arena = self._arena
-        waiting = eng.waiting() if getattr(eng, "waiting", None) is not None else None
-        eng.waiting = None
-        if waiting is not None and waiting.format is not None:   # (set_train_checkpoints: an earlier forward's graph still lives)
-            waiting.checkpoint = eng.checkpoint_save(waiting.format)
+        _displace(eng)
         eng.refresh(arena.flat)                       # weight blocks + PReLU tables; BN tables are rewritten per batch
         units, _, names = self._desc_cache(arena)
         self._flop_tab = self._flop_weight_table(names, units)
@@ -672,9 +669,7 @@ class _CSNetTrainFn(torch.autograd.Function):
         if eng.waiting is not None and eng.waiting() is s:
             pass
         elif s.checkpoint is not None:
-            eng.waiting, waiting = None, eng.waiting() if eng.waiting is not None else None
-            if waiting is not None:                     # the workspace holds another forward that still waits: out of the way
-                waiting.checkpoint = eng.checkpoint_save(waiting.format)
+            _displace(eng)                              # the workspace may hold another forward that still waits
             eng.checkpoint_restore(s.checkpoint, s.format)
             model._train_generation += 1                # (a forward without checkpoints in between is gone, too)
         else:
@@ -702,6 +697,14 @@ class _SavedForward:
         # float32 steps read the image batch again in the backward (bfloat16 ones keep a copy of their own, which is saved)
         self.x_version = None if self.engine.train_bf16 or x.is_inference() else x._version
         self.engine.waiting = weakref.ref(self)
+
+
+def _displace(eng):
+    """Make room in a plan's workspace: the forward that lies there and waits for its backward, if there is one, is saved."""
+    waiting = eng.waiting() if getattr(eng, "waiting", None) is not None else None
+    if waiting is not None:
+        waiting.checkpoint = eng.checkpoint_save(waiting.format)   # (where this fails, out of memory say, it still lies there)
+    eng.waiting = None
 
 
 def _versions(model):

@@ -28,3 +28,7 @@ def test_gpu_two_streams(lib, x2_manifest, act_dtype):
 
 def test_gpu_changed_parameters(lib, x2_manifest):
     W.check_changed_parameters(lib, DEV, x2_manifest)
+
+
+def test_gpu_failed_save(lib, x2_manifest):
+    W.check_failed_save(lib, DEV, x2_manifest)

@@ -81,3 +81,7 @@ def test_uses_of_the_workspace_wait_for_each_other(lib, x2_manifest, monkeypatch
 
 def test_emu_changed_parameters(lib, x2_manifest):
     W.check_changed_parameters(lib, CPU, x2_manifest)
+
+
+def test_emu_failed_save(lib, x2_manifest):
+    W.check_failed_save(lib, CPU, x2_manifest)

@@ -113,3 +113,30 @@ def check_changed_parameters(lib, device, manifest):
             b = m(other)
         a.backward(dy)
         assert torch.equal(grads(m), want)
+
+
+def check_failed_save(lib, device, manifest):
+    """The checkpoint that would make room for the next forward cannot be had (out of memory): that forward raises and the one that
+    waits keeps its place, exact gradients included; so it does where an older forward's backward wanted the room."""
+    xs = [batch(s, device) for s in (31, 32)]
+    dy = K.gradient((1, 1, 16, 16), torch.float32, 1, device)
+    m = net(lib, device, manifest)
+    m(xs[1]).backward(dy)
+    exact = grads(m)
+    eng = m.engine_for(xs[0], train=True)
+    save = eng.checkpoint_save
+
+    def fails(format):
+        raise torch.OutOfMemoryError("no room")
+    a, b = m(xs[0]), m(xs[1])
+    eng.checkpoint_save = fails
+    with pytest.raises(torch.OutOfMemoryError):
+        m(xs[0])
+    with pytest.raises(torch.OutOfMemoryError):
+        a.backward(dy)
+    eng.checkpoint_save = save
+    m.zero_grad(set_to_none=True)
+    b.backward(dy)
+    assert torch.equal(grads(m), exact)
+    a.backward(dy)
+    assert bool(torch.isfinite(grads(m)).all())
