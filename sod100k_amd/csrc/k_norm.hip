@@ -110,7 +110,7 @@ static unsigned norm_grid(int64_t items) { return (unsigned)(items < 16384 ? ite
 enum { NORM_X = -1 };   // input of the backward: x itself (else a checkpoint format); forward: no checkpoint is written
 
 // sums over G lanes (a power of two): a butterfly inside the wave, then the block's waves in order through LDS (two buffers of
-// [N][16] floats in turn: one barrier per sum)
+// [2][16] floats in turn: one barrier per sum)
 template <int G, int N>
 __device__ __forceinline__ void norm_sum(float (&v)[N], float* sm, int& turn) {
 #pragma unroll
@@ -123,7 +123,8 @@ __device__ __forceinline__ void norm_sum(float (&v)[N], float* sm, int& turn) {
     v[i] += csn_lane_xor_f32<1>(v[i]);
   }
   if (G > 64) {
-    float* b = sm + turn * (N * 16);
+    static_assert(N <= 2, "a buffer holds two sums");
+    float* b = sm + turn * 32;
     turn ^= 1;
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
@@ -157,6 +158,22 @@ __device__ __forceinline__ void norm_param(float (&f)[E], const float* p, int n,
 #pragma unroll
     for (int j = 0; j < 4; ++j) f[h + j] = p && h + j < n ? csn_bits_f(v.w[j]) : none;
   }
+}
+
+// A float sum leaves a mean m off by some of its last places; the second pass, over x - m, finds out by how much.
+// The product that gives m must not be contracted with the subtraction: what is taken off would not be m.
+__device__ __forceinline__ float norm_first_mean(float sum, float inv_c) {
+  unsigned m = csn_f_bits(sum * inv_c);
+  csn_pin(m);
+  return csn_bits_f(m);
+}
+// From the sums of (x - m)^2 and of x - m: the variance, and m becomes the mean.  (Equal channels: x - m is the same few last places of x for
+// all of them; sums, the quotient -- corrected once, a division at less cost -- and the difference are exact: mean x, variance 0.)
+__device__ __forceinline__ float norm_correct(float& m, float sq, float sum, float channels, float inv_c) {
+  const float q = sum * inv_c, off = fmaf(fmaf(-q, channels, sum), inv_c, q);
+  m += off;
+  const float var = fmaf(-off, sum, sq) * inv_c;
+  return var < 0.f ? 0.f : var;   // (a NaN stays one)
 }
 
 template <int G> struct NormRowsBlock { static constexpr int T = G > CSN_BLOCK ? G : CSN_BLOCK; };
@@ -203,8 +220,7 @@ __global__ __launch_bounds__(NormRowsBlock<G>::T) void norm_rows_fwd_kernel(Norm
       for (int j = 0; j < E; ++j) s[0] += f[j];
     }
     norm_sum<G, 1>(s, sm, turn);
-    const float mean = s[0] / (float)C;   // (divided: equal channels have no variance at all)
-    s[0] = 0.f;
+    float mean = norm_first_mean(s[0], inv_c), d2[2] = {0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       float f[E];
@@ -213,11 +229,13 @@ __global__ __launch_bounds__(NormRowsBlock<G>::T) void norm_rows_fwd_kernel(Norm
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         const float d = j < n[v] ? f[j] - mean : 0.f;
-        s[0] = fmaf(d, d, s[0]);
+        d2[0] = fmaf(d, d, d2[0]);
+        d2[1] += d;
       }
     }
-    norm_sum<G, 1>(s, sm, turn);
-    const float rstd = 1.f / sqrtf(fmaf(s[0], inv_c, a.eps));
+    norm_sum<G, 2>(d2, sm, turn);
+    const float var = norm_correct(mean, d2[0], d2[1], (float)C, inv_c);
+    const float rstd = 1.f / sqrtf(var + a.eps);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int c0 = E * (l + G * v);
@@ -367,7 +385,7 @@ __global__ __launch_bounds__(NormRowsBlock<G>::T) void norm_rows_bwd_kernel(Norm
 
 // Planar maps: PX lanes along the pixels (four consecutive pixels of a channel per lane: eight would double the statistics that
 // every lane carries), T / PX groups of lanes over the channels, NC channels per lane in registers.  Sums over a pixel's channels: butterfly over the groups of a wave, then the waves in
-// order through LDS (two buffers of [waves][N][PX * E] floats in turn).
+// order through LDS (two buffers of [waves][2][PX * E] floats in turn).
 #define NORM_PE 4
 template <int T, int PX, int E, int N>
 __device__ __forceinline__ void norm_planar_sum(float (&v)[N][E], float* sm, int& turn) {
@@ -383,7 +401,8 @@ __device__ __forceinline__ void norm_planar_sum(float (&v)[N][E], float* sm, int
       if (PX <= 2) v[i][j] += csn_lane_xor_f32<2>(v[i][j]);
     }
   if (W == 1) return;
-  float* b = sm + turn * (W * N * TP);
+  static_assert(N <= 2, "a buffer holds two sums");
+  float* b = sm + turn * (W * 2 * TP);
   turn ^= 1;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, px = lane % PX;
   if (lane < PX)
@@ -412,8 +431,9 @@ __device__ __forceinline__ T* norm_at(T* base, unsigned bytes) {
 }
 // A block's items: first, first + step, ... below end.  Where tiles are not whole cache lines of the map, each XCD (block b runs on XCD b % 8, the
 // grid is a multiple of 8) takes a run of neighbouring tiles, so that the lines that their edges cut are read once into one L2; whole lines
-// lose a few percent that way.  Backward, round robin / runs, us: 16x512x44x44 bf16 40.5 / 29.4, 16x2048x28x28 bf16 158 / 68, 32x256x57x57
-// bf16 60.2 / 45.6; of whole lines 32x256x88x88 bf16 94.2 / 97.2, 32x128x88x88 float 81.3 / 85.4.
+// lose a few percent that way.  Round robin / runs, us, backward: 16x512x44x44 bf16 40.5 / 29.4, 16x2048x28x28 bf16 158 / 68, 32x256x57x57
+// bf16 60.2 / 45.6; of whole lines 32x256x88x88 bf16 94.2 / 97.2, 32x128x88x88 float 81.3 / 85.4.  Forward: 16x512x44x44 bf16 18.2 / 16.1, float
+// 30.0 / 29.4, 16x2048x28x28 bf16 41.6 / 35.7, 32x256x57x57 bf16 40.7 / 29.3, float with a checkpoint 87.4 / 64.8.
 struct NormItems { int first, step, end; };
 __device__ __forceinline__ NormItems norm_items(const NormArgs& a) {
   const int b = blockIdx.x, grid = gridDim.x;
@@ -428,7 +448,7 @@ __device__ __forceinline__ void norm_load(VecIo<AT, E>& v, const AT* base, unsig
   if (n > 0) v.load(norm_at(base, bytes));
 }
 // (Four waves per SIMD: a float form with a checkpoint gives up ten registers for a second block of 512 threads on the CU, 16x512x44x44
-// 35.2 -> 31.9 us.)
+// 37.5 -> 34.1 us, 32x256x57x57 61.2 -> 58.9.)
 template <typename AT, int T, int PX, int NC, int CK>
 __global__ __launch_bounds__(T, 4) void norm_planar_fwd_kernel(NormArgs a) {
   constexpr int E = NORM_PE, CG = T / PX, TP = PX * E;
@@ -470,9 +490,32 @@ __global__ __launch_bounds__(T, 4) void norm_planar_fwd_kernel(NormArgs a) {
       CSN_SCHED_FENCE();   // one channel's floats at a time in registers
     }
     norm_planar_sum<T, PX, E, 1>(s, sm, turn);
+    // (As above; both sums of the second pass at once where the registers hold them.  float, whose channels take twice as many, would
+    // spill and corrects the mean in a pass of its own: at once / in turn, us, bf16 32x256x88x88 47.7 / 50.3, 16x512x44x44 16.1 / 17.0;
+    // float 16x2048x28x28 57.2 / 51.9, 16x1024x32x32 34.0 / 29.9, 32x256x88x88 107.6 / 105.4.)
+    constexpr bool ONCE = sizeof(AT) == 2;
     float mean[E], rstd[E];
 #pragma unroll
-    for (int j = 0; j < E; ++j) { mean[j] = s[0][j] / (float)C; s[0][j] = 0.f; }   // (divided: as above)
+    for (int j = 0; j < E; ++j) mean[j] = norm_first_mean(s[0][j], inv_c);
+    if constexpr (!ONCE) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) s[0][j] = 0.f;
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        float f[E];
+        r[k].pin();
+        r[k].get(f);
+#pragma unroll
+        for (int j = 0; j < E; ++j) s[0][j] += cg + CG * k < C ? f[j] - mean[j] : 0.f;
+        CSN_SCHED_FENCE();
+      }
+      norm_planar_sum<T, PX, E, 1>(s, sm, turn);
+#pragma unroll
+      for (int j = 0; j < E; ++j) mean[j] = fmaf(s[0][j], inv_c, mean[j]);
+    }
+    float d2[ONCE ? 2 : 1][E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) d2[0][j] = d2[ONCE][j] = 0.f;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       float f[E];
@@ -481,13 +524,17 @@ __global__ __launch_bounds__(T, 4) void norm_planar_fwd_kernel(NormArgs a) {
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         const float d = cg + CG * k < C ? f[j] - mean[j] : 0.f;
-        s[0][j] = fmaf(d, d, s[0][j]);
+        d2[0][j] = fmaf(d, d, d2[0][j]);
+        if (ONCE) d2[ONCE][j] += d;
       }
       CSN_SCHED_FENCE();
     }
-    norm_planar_sum<T, PX, E, 1>(s, sm, turn);
+    norm_planar_sum<T, PX, E, ONCE ? 2 : 1>(d2, sm, turn);
 #pragma unroll
-    for (int j = 0; j < E; ++j) rstd[j] = 1.f / sqrtf(fmaf(s[0][j], inv_c, a.eps));
+    for (int j = 0; j < E; ++j) {
+      const float var = ONCE ? norm_correct(mean[j], d2[0][j], d2[ONCE][j], (float)C, inv_c) : d2[0][j] * inv_c;
+      rstd[j] = 1.f / sqrtf(var + a.eps);
+    }
     const int64_t row0 = (int64_t)o * C;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
@@ -721,7 +768,7 @@ static int norm_rows_run(const NormArgs& a, const NormPlan& p, bool bwd, void* s
 }
 template <typename AT, int T, int PX, int NC, int CK>
 static int norm_planar_fwd(const NormArgs& a, void* stream) {
-  const size_t sm = (size_t)2 * (T / 64) * PX * NORM_PE * sizeof(float);
+  const size_t sm = (size_t)2 * (T / 64) * 2 * PX * NORM_PE * sizeof(float);
   CSN_LAUNCH((norm_planar_fwd_kernel<AT, T, PX, NC, CK>), dim3((unsigned)a.slabs), dim3(T), sm, stream, a);
   return (int)hipGetLastError();
 }

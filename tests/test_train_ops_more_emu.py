@@ -1,0 +1,22 @@
+"""Further checks of the training operators beside the plan on the CPU emulation of their kernels (lane-exact mode)."""
+import pytest
+import torch
+
+import train_ops_cases as K
+import train_ops_more as M
+
+
+@pytest.fixture(scope="module")
+def lib(emu_lanes_lib):
+    return emu_lanes_lib[0]
+
+
+@pytest.mark.parametrize("dtype", K.DTYPES)
+@pytest.mark.parametrize("shape,dim", M.CONSTANT)
+def test_emu_constant_tokens(lib, shape, dim, dtype):
+    M.check_constant_tokens(lib, "cpu", shape, dim, dtype)
+
+
+@pytest.mark.parametrize("shape,dim", [((3, 100), -1), ((2, 40, 3, 5), 1)])
+def test_emu_nan_statistics(lib, shape, dim):
+    M.check_nan_statistics(lib, "cpu", shape, dim)
