@@ -184,8 +184,6 @@ def _dense_like(x: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
 
 
-
-
 def layer_norm_forward(lib: C.CDLL, x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                        dim: int = -1, eps: float = 1e-5, checkpoint: Optional[str] = None
                        ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, Optional[Q8]]:
@@ -291,11 +289,15 @@ def _refuse_capture() -> None:
                            "*_weight_grad functions instead")
 
 
+def _records(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether autograd records an operator on these tensors: where it does not, nothing is kept for a backward pass."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, lib, x, weight, bias, dim, eps, checkpoint):
-        if any(ctx.needs_input_grad):
-            _refuse_capture()
+        _refuse_capture()
         y, mean, rstd, q = layer_norm_forward(lib, x, weight, bias, dim=dim, eps=eps, checkpoint=checkpoint)
         ctx.lib, ctx.dim = lib, dim
         if q is None:
@@ -320,8 +322,14 @@ class _LayerNormFn(torch.autograd.Function):
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, dim: int = -1,
                eps: float = 1e-5, checkpoint: Optional[str] = None, lib: Optional[C.CDLL] = None) -> torch.Tensor:
     """Differentiable layer norm over axis ``dim``.  ``checkpoint`` ("int8" / "e4m3") keeps x for the backward in 8 bits instead of
-    the tensor itself: the gradients are then those of the checkpoint's values."""
-    return _LayerNormFn.apply(lib or N.load(), x, weight, bias, dim, eps, checkpoint)
+    the tensor itself: the gradients are then those of the checkpoint's values.  Without gradients (``torch.no_grad()``) nothing is
+    kept, and the call may be captured."""
+    lib = lib or N.load()
+    if not _records(x, weight, bias):
+        if checkpoint is not None:
+            _format(checkpoint)
+        return layer_norm_forward(lib, x, weight, bias, dim=dim, eps=eps)[0]
+    return _LayerNormFn.apply(lib, x, weight, bias, dim, eps, checkpoint)
 
 
 def _product(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], rows: bool) -> torch.Tensor:
@@ -339,27 +347,29 @@ def _product(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor]
 class _ProductFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, lib, x, weight, bias, dim, checkpoint):
-        if any(ctx.needs_input_grad):
-            _refuse_capture()
+        _refuse_capture()
         rows = _channel_axis(dim, x.dim())
         y = _product(x, weight, bias, rows)
         ctx.lib, ctx.dim, ctx.rows = lib, dim, rows
-        q = q8_pack(lib, x, checkpoint, start_dim=-1 if rows else 2)
-        ctx.q = (q.format, q.start_dim)
-        ctx.save_for_backward(weight, q.codes, q.scales)
+        if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
+            q = q8_pack(lib, x, checkpoint, start_dim=-1 if rows else 2)
+            ctx.q = (q.format, q.start_dim)
+            ctx.save_for_backward(weight, q.codes, q.scales)
+        else:
+            ctx.save_for_backward(weight)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         _refuse_capture()
-        weight, codes, scales = ctx.saved_tensors
+        weight, *kept = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dw = db = None
         if need[1]:
             dx = _product(dy, weight.t().contiguous(), None, ctx.rows)
         if need[2] or need[3]:
-            dw, db = product_weight_grad(ctx.lib, dy, Q8(codes, scales, *ctx.q), dim=ctx.dim)
+            dw, db = product_weight_grad(ctx.lib, dy, Q8(*kept, *ctx.q), dim=ctx.dim)
         return None, dx, dw if need[2] else None, db if need[3] else None, None, None
 
 
@@ -367,9 +377,16 @@ def product(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] 
             lib: Optional[C.CDLL] = None) -> torch.Tensor:
     """Differentiable 1x1 convolution over planar maps (``dim=1``) or linear layer over rows (``dim=-1``), weight [Cout, Cin], that
     keeps its input for the weight gradient as an 8-bit checkpoint.  The forward and the input gradient are exact library products
-    in x's dtype; only the weight gradient sees the checkpoint's values."""
+    in x's dtype; only the weight gradient sees the checkpoint's values.  Without gradients (``torch.no_grad()``) nothing is kept, and
+    the call may be captured."""
+    lib = lib or N.load()
     ch = x.shape[-1] if _channel_axis(dim, x.dim()) else x.shape[1]
     if weight.dim() != 2 or weight.shape[1] != ch or weight.dtype != torch.float32:
         raise ValueError(f"weight: float32 of shape (Cout, {ch}) expected, got {weight.dtype} {tuple(weight.shape)}")
     bias = _param(bias, weight.shape[0], "bias")
-    return _ProductFn.apply(lib or N.load(), x, weight, bias, dim, checkpoint)
+    _dtype(x, "product")
+    _format(checkpoint)
+    _same_device(lib, x, weight, bias)
+    if not _records(x, weight, bias):
+        return _product(x, weight, bias, _channel_axis(dim, x.dim()))
+    return _ProductFn.apply(lib, x, weight, bias, dim, checkpoint)

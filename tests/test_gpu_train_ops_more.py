@@ -26,3 +26,29 @@ def test_gpu_constant_tokens(lib, shape, dim, dtype):
 @pytest.mark.parametrize("shape,dim", [((3, 100), -1), ((2, 40, 3, 5), 1)])
 def test_gpu_nan_statistics(lib, shape, dim):
     M.check_nan_statistics(lib, DEV, shape, dim)
+
+
+def test_gpu_without_gradients(lib, monkeypatch):
+    M.check_without_gradients(lib, DEV, monkeypatch)
+
+
+def test_gpu_captured_without_gradients(lib):
+    """An inference pass of the differentiable forms, parameters included, captured and replayed between eager work."""
+    x = K.activations((40, 64), torch.bfloat16, 1, DEV)
+    w, b = (torch.nn.Parameter(p) for p in K.params(64, 1, DEV))
+    W = torch.nn.Parameter(torch.randn(32, 64, generator=torch.Generator().manual_seed(2)).to(DEV))
+
+    def run():
+        with torch.no_grad():
+            return T.product(T.layer_norm(x, w, b, checkpoint="int8"), W)
+    want = run()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = run()
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        assert torch.equal(run(), want)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)

@@ -20,3 +20,7 @@ def test_emu_constant_tokens(lib, shape, dim, dtype):
 @pytest.mark.parametrize("shape,dim", [((3, 100), -1), ((2, 40, 3, 5), 1)])
 def test_emu_nan_statistics(lib, shape, dim):
     M.check_nan_statistics(lib, "cpu", shape, dim)
+
+
+def test_emu_without_gradients(lib, monkeypatch):
+    M.check_without_gradients(lib, "cpu", monkeypatch)

@@ -31,3 +31,43 @@ def check_nan_statistics(lib, dev, shape, dim):
         z.select(dim, 1).fill_(bad)
         _, mean, rstd, _ = T.layer_norm_forward(lib, z, dim=dim)
         assert not bool(torch.isfinite(mean).any()) and bool(torch.isnan(rstd).all())
+
+
+def check_without_gradients(lib, dev, monkeypatch):
+    """Under no_grad and inference_mode, parameters or not, the differentiable forms return the same values and keep nothing; where the
+    input of a product alone wants a gradient, none of it is kept either."""
+    packs = []
+    real = T._launch
+
+    def launch(lib, device, what, *args):
+        packs.append(what == "csn_q8_pack" or (what == "csn_layer_norm_forward" and args[-1] is not None))
+        real(lib, device, what, *args)
+    monkeypatch.setattr(T, "_launch", launch)
+    g = torch.Generator().manual_seed(1)
+    for shape, dim in (((5, 16), -1), ((2, 16, 3, 3), 1)):
+        x = torch.randn(shape, generator=g).to(dev)
+        w, b = (torch.nn.Parameter(p) for p in K.params(16, 1, dev))
+        W = torch.nn.Parameter(torch.randn(8, 16, generator=g).to(dev))
+        c = torch.nn.Parameter(torch.randn(8, generator=g).to(dev))
+        norm = lambda: T.layer_norm(x, w, b, dim=dim, checkpoint="int8", lib=lib)
+        prod = lambda: T.product(x, W, c, dim=dim, lib=lib)
+        want = norm().detach(), prod().detach()
+        assert any(packs)
+        for mode in (torch.no_grad, torch.inference_mode):
+            del packs[:]
+            with mode():
+                got = norm(), prod()
+                for call in (lambda: T.layer_norm(x, w, b, dim=dim, checkpoint="fp4", lib=lib), lambda: T.product(x, W, c, dim=dim, checkpoint="fp4", lib=lib)):
+                    with pytest.raises(ValueError):
+                        call()
+                with pytest.raises(TypeError):
+                    T.product(x.half(), W, c, dim=dim, lib=lib)
+            for p, q in zip(got, want):
+                assert torch.equal(p, q) and not p.requires_grad
+            assert not any(packs)
+        z = x.clone().requires_grad_()
+        del packs[:]
+        T.product(z, W.detach(), c.detach(), dim=dim, lib=lib).sum().backward()
+        assert not any(packs)
+        tok = W.detach().sum(0)
+        assert torch.allclose(z.grad, (tok if dim == -1 else tok.view(1, -1, 1, 1)).expand(shape), rtol=64 * K.U * 8, atol=64 * K.U * 8)
