@@ -213,10 +213,11 @@ def layer_norm_forward(lib: C.CDLL, x: torch.Tensor, weight: Optional[torch.Tens
 
 
 def layer_norm_backward(lib: C.CDLL, dy: torch.Tensor, x: Union[torch.Tensor, Q8], mean: torch.Tensor, rstd: torch.Tensor,
-                        weight: Optional[torch.Tensor] = None, dim: int = -1
-                        ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                        weight: Optional[torch.Tensor] = None, dim: int = -1, param_grads: bool = True
+                        ) -> Tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
     """``(dx, dweight, dbias)`` of a layer norm from its input ``x`` -- the tensor or its checkpoint -- and the statistics of the
-    forward.  ``dx`` is dense in dy's dtype, the parameter gradients float32."""
+    forward.  ``dx`` is dense in dy's dtype, the parameter gradients float32; ``param_grads=False`` leaves them out (None): a frozen
+    norm's backward is one launch."""
     dt = _dtype(dy, "layer_norm")
     rows = _channel_axis(dim, dy.dim())
     ch = dy.shape[-1] if rows else dy.shape[1]
@@ -238,10 +239,13 @@ def layer_norm_backward(lib: C.CDLL, dy: torch.Tensor, x: Union[torch.Tensor, Q8
     dev = _same_device(lib, dy, src, q.scales if q is not None else None, mean, rstd, weight)
     d = _norm_desc(rows, dt, dy.shape, 1.0, fmt)
     dx = _dense_like(dy)
-    dweight = dy.new_empty((ch,), dtype=torch.float32)
-    dbias = dy.new_empty((ch,), dtype=torch.float32)
-    nbytes = lib.csn_layer_norm_workspace_bytes(C.byref(d))
-    ws = dy.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
+    dweight = dbias = ws = None
+    nbytes = 0
+    if param_grads:
+        dweight = dy.new_empty((ch,), dtype=torch.float32)
+        dbias = dy.new_empty((ch,), dtype=torch.float32)
+        nbytes = lib.csn_layer_norm_workspace_bytes(C.byref(d))
+        ws = dy.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
     vd, dso, dsc = _view(dy, rows) if dy.numel() else (dy, 0, 0)
     vx, so, sc, codes, scales = None, 0, 0, None, None
     if dy.numel():
@@ -250,7 +254,7 @@ def layer_norm_backward(lib: C.CDLL, dy: torch.Tensor, x: Union[torch.Tensor, Q8
         else:
             codes, scales = q.codes.data_ptr(), q.scales.data_ptr()
     _launch(lib, dev, "csn_layer_norm_backward", C.byref(d), vd.data_ptr(), dso, dsc, _ptr(vx), so, sc, codes, scales, mean.data_ptr(),
-            rstd.data_ptr(), _ptr(weight), dx.data_ptr(), dweight.data_ptr(), dbias.data_ptr(), _ptr(ws), nbytes)
+            rstd.data_ptr(), _ptr(weight), dx.data_ptr(), _ptr(dweight), _ptr(dbias), _ptr(ws), nbytes)
     return dx, dweight, dbias
 
 
@@ -314,8 +318,8 @@ class _LayerNormFn(torch.autograd.Function):
         _refuse_capture()
         mean, rstd, weight, *src = ctx.saved_tensors
         x = src[0] if ctx.q is None else Q8(src[0], src[1], *ctx.q)
-        dx, dw, db = layer_norm_backward(ctx.lib, dy, x, mean, rstd, weight, dim=ctx.dim)
         need = ctx.needs_input_grad
+        dx, dw, db = layer_norm_backward(ctx.lib, dy, x, mean, rstd, weight, dim=ctx.dim, param_grads=need[2] or need[3])
         return None, dx if need[1] else None, dw if need[2] else None, db if need[3] else None, None, None, None
 
 

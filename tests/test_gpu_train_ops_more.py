@@ -52,3 +52,7 @@ def test_gpu_captured_without_gradients(lib):
         assert torch.equal(run(), want)
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+def test_gpu_frozen_norm(lib, monkeypatch):
+    M.check_frozen_norm(lib, DEV, monkeypatch)

@@ -24,3 +24,7 @@ def test_emu_nan_statistics(lib, shape, dim):
 
 def test_emu_without_gradients(lib, monkeypatch):
     M.check_without_gradients(lib, "cpu", monkeypatch)
+
+
+def test_emu_frozen_norm(lib, monkeypatch):
+    M.check_frozen_norm(lib, "cpu", monkeypatch)

@@ -71,3 +71,31 @@ def check_without_gradients(lib, dev, monkeypatch):
         assert not any(packs)
         tok = W.detach().sum(0)
         assert torch.allclose(z.grad, (tok if dim == -1 else tok.view(1, -1, 1, 1)).expand(shape), rtol=64 * K.U * 8, atol=64 * K.U * 8)
+
+
+def check_frozen_norm(lib, dev, monkeypatch):
+    """The backward of a norm whose parameters want no gradient asks for none: the same dx, no workspace, no second launch."""
+    asked = []
+    real = T._launch
+
+    def launch(lib, device, what, *args):
+        if what == "csn_layer_norm_backward":
+            asked.append([a is not None for a in args[-4:]])      # dweight, dbias, workspace, its size
+        real(lib, device, what, *args)
+    monkeypatch.setattr(T, "_launch", launch)
+    for shape, dim in (((3000, 16), -1), ((2, 16, 30, 30), 1)):
+        for ck in (None, "int8"):
+            x0, dy = K.activations(shape, torch.float32, 1, dev, rows=dim == -1), K.gradient(shape, torch.float32, 1, dev)
+            w, b = K.params(16, 1, dev)
+            dx = []
+            for train in (True, False):
+                del asked[:]
+                x = x0.clone().requires_grad_()
+                wt, bt = (t.clone().requires_grad_(train) for t in (w, b))
+                T.layer_norm(x, wt, bt, dim=dim, checkpoint=ck, lib=lib).backward(dy)
+                dx.append(x.grad)
+                assert asked == [[train, train, train, True]]
+                assert (wt.grad is not None) == train and (bt.grad is not None) == train
+            assert torch.equal(*dx)
+    _, mean, rstd, _ = T.layer_norm_forward(lib, x0, w, b, dim=1)
+    assert T.layer_norm_backward(lib, dy, x0, mean, rstd, w, dim=1, param_grads=False)[1:] == (None, None)
