@@ -337,7 +337,10 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
 
 def _product(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], rows: bool) -> torch.Tensor:
-    """The forward product itself: one library matrix product in x's dtype."""
+    """The forward product itself: one library matrix product in x's dtype, whatever autocast would make of it."""
+    if torch.is_autocast_enabled(x.device.type):
+        with torch.autocast(x.device.type, enabled=False):
+            return _product(x, weight, bias, rows)
     w = weight.to(x.dtype)
     b = None if bias is None else bias.to(x.dtype)
     if rows:

@@ -56,3 +56,7 @@ def test_gpu_captured_without_gradients(lib):
 
 def test_gpu_frozen_norm(lib, monkeypatch):
     M.check_frozen_norm(lib, DEV, monkeypatch)
+
+
+def test_gpu_autocast(lib):
+    M.check_autocast(lib, DEV)

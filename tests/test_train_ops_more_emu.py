@@ -28,3 +28,7 @@ def test_emu_without_gradients(lib, monkeypatch):
 
 def test_emu_frozen_norm(lib, monkeypatch):
     M.check_frozen_norm(lib, "cpu", monkeypatch)
+
+
+def test_emu_autocast(lib):
+    M.check_autocast(lib, "cpu")

@@ -99,3 +99,24 @@ def check_frozen_norm(lib, dev, monkeypatch):
             assert torch.equal(*dx)
     _, mean, rstd, _ = T.layer_norm_forward(lib, x0, w, b, dim=1)
     assert T.layer_norm_backward(lib, dy, x0, mean, rstd, w, dim=1, param_grads=False)[1:] == (None, None)
+
+
+def check_autocast(lib, dev):
+    """Inside autocast the product stays in its input's dtype, forward and backward: bit for bit what it is outside."""
+    g = torch.Generator().manual_seed(1)
+    kind = torch.device(dev).type
+    for shape, dim in (((6, 16), -1), ((2, 16, 3, 3), 1)):
+        x0, W0, c0 = (torch.randn(s, generator=g).to(dev) for s in (shape, (8, 16), (8,)))
+        res = []
+        for half in (None, torch.bfloat16, torch.float16):
+            x, W, c = (t.clone().requires_grad_() for t in (x0, W0, c0))
+            with torch.autocast(kind, dtype=half or torch.bfloat16, enabled=half is not None):
+                y = T.product(x, W, c, dim=dim, lib=lib)
+                with torch.no_grad():
+                    assert torch.equal(T.product(x, W, c, dim=dim, lib=lib), y)
+                y.sum().backward()
+            assert y.dtype == torch.float32
+            res.append((y.detach(), x.grad, W.grad, c.grad))
+        for r in res[1:]:
+            for p, q in zip(res[0], r):
+                assert torch.equal(p, q)
