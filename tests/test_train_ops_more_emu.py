@@ -32,3 +32,20 @@ def test_emu_frozen_norm(lib, monkeypatch):
 
 def test_emu_autocast(lib):
     M.check_autocast(lib, "cpu")
+
+
+def test_refusals_of_workspaces(lib):
+    M.check_refusals_of_workspaces(lib)
+
+
+def test_refusals_of_workspaces_of_the_product_library():
+    import ctypes
+    import os
+    from sod100k_amd import _native as N
+    if not os.path.exists(N.LIB_PATH):
+        pytest.skip("libcsnet_hip.so not built")
+    M.check_refusals_of_workspaces(N.bind(ctypes.CDLL(N.LIB_PATH)))
+
+
+def test_emu_outputs_end_where_they_end(lib):
+    M.check_outputs_end_where_they_end(lib, "cpu")

@@ -140,3 +140,31 @@ def check_failed_save(lib, device, manifest):
     assert torch.equal(grads(m), exact)
     a.backward(dy)
     assert bool(torch.isfinite(grads(m)).all())
+
+
+def check_penalty_and_input_gradients(lib, device, manifest, act_dtype, B=2, size=16):
+    """A loss over two forwards with the penalty in it, both batches wanting their gradient: the older forward's gradients are those of
+    its checkpoint, the newer one's exact, as the plan's own calls give them."""
+    from sod100k_amd import _native as N
+    xs = [batch(s, device, B, size) for s in (31, 32)]
+    dy = K.gradient((B, 1, size, size), torch.float32, 1, device)
+    scale = 0.25
+
+    def alone(x, through_checkpoint):
+        m = K._net(lib, device, manifest, act_dtype, B)
+        m._want_input_grad = True
+        m._train_forward_raw(x)
+        eng = m.engine_for(x, train=True)
+        if through_checkpoint:
+            eng.checkpoint_restore(eng.checkpoint_save(N.Q8_INT8), N.Q8_INT8)
+        g = m._train_backward_raw(x, dy, scale).clone()
+        return torch.cat([g[m._arena.offsets[n]:m._arena.offsets[n] + p.numel()] for n, p in m.named_parameters()]), eng.train_probe(0, "grad0")
+    (g0, dx0), (g1, dx1) = alone(xs[0], True), alone(xs[1], False)
+    m = net(lib, device, manifest, act_dtype, B=B)
+    m.clear_flops()
+    leaves = [x.clone().requires_grad_() for x in xs]
+    a, b = (m(x) for x in leaves)
+    ((a * dy).sum() + (b * dy).sum() + scale * B * m.get_flops()).backward()
+    assert torch.equal(leaves[0].grad, dx0) and torch.equal(leaves[1].grad, dx1)
+    assert torch.equal(grads(m), g1 + g0)
+    assert bool(dx0.abs().sum() > 0) and not torch.equal(g0, g1)
