@@ -23,7 +23,9 @@
 // alone are 20.8 at the rate of a copy and the multiplications 14: no single part holds it (with steps of 64 tokens, 57 with the sum: 50
 // without the exponents' loads, 45 without X's or without dY's, 53 without multiplying, 55 without decoding).  16384 tokens,
 // 1024 -> 4096 channels, bf16: 177 (+15.7), 776 TFLOP/s of matrix instructions against 841 of the library's product of two bf16 tensors of
-// these sizes.  37 -> 21 channels over 5x13x17 float 7.8 (+1.9).
+// these sizes.  37 -> 21 channels over 5x13x17 float 7.8 (+1.9).  float dY, with the sum, of the floor (three times the bf16 operations):
+// 16384 tokens, 1024 -> 4096 632 of 347, 512 -> 512 50.6 of 21.7, 32x88x88, 256 -> 128 95.5 of 41.0: one wave per SIMD (the three parts fill
+// the LDS), so that cutting and multiplying take turns.
 #include "q8_core.h"
 #include "slab_sum.h"
 #include "train_ops.h"
@@ -424,8 +426,10 @@ struct WgPlan { int tm, tn, mtiles, ntiles, steps_per_slab, slabs, chunks; };
 // Tiles of 128 where the channels fill more than 64; of 256 x 256, whose operands are read from LDS half as often, where there are enough of
 // them times steps for every CU (bfloat16 dY: the three parts of a float one do not fit).  Tiles of 128 / of 256, us with the sum of the
 // slabs: 16384 tokens, 1024 -> 4096 245 / 172, 1024 -> 1024 72 / 64, 512 -> 512 32 / 36; 2048 tokens, 1024 -> 4096 50 / 46; 131072 tokens,
-// 256 -> 256 45 / 46, 65536 tokens 32 / 37.  About one block of eight waves or two of four
-// per CU, but at least 256 tokens each: a slab costs a partial tile written and read again.
+// 256 -> 256 45 / 46, 65536 tokens 32 / 37.  As many blocks as the CUs hold at a time, but at least 256 tokens each: a slab costs a partial
+// tile written and read again.  A CU holds one block of eight waves or two of four, and one of four where the three parts of a float dY of
+// 128 channels fill its LDS; two rounds of those / one, us: 16384 tokens, 512 -> 512 58.4 / 50.6, 32768 tokens, 256 -> 256 41.4 / 32.6,
+// 32x44x44 maps, 256 -> 256 60.4 / 51.6, 32x88x88, 256 -> 128 101.2 / 95.5.
 static bool wg_plan(int rows, int a16, int64_t outer, int64_t inner, int64_t cin, int64_t cout, WgPlan& p) {
   const int64_t chunks = rows ? 1 : (inner + 7) / 8, per_step = !rows && a16 ? 16 : 8;
   const int64_t all = rows ? (outer + 7) / 8 : outer * chunks, steps = (all + per_step - 1) / per_step;
@@ -435,8 +439,8 @@ static bool wg_plan(int rows, int a16, int64_t outer, int64_t inner, int64_t cin
   if (big) p.tm = p.tn = 256;
   const int64_t mt = (cout + p.tm - 1) / p.tm, nt = (cin + p.tn - 1) / p.tn;
   if (mt * nt > (1 << 20) || all > 0x7ffffe00LL || chunks > 0x7ffffe00LL) return false;
-  const bool eight = big || (per_step == 16 && p.tm + p.tn > 128);
-  int64_t slabs = ((eight ? 256 : 512) + mt * nt - 1) / (mt * nt);
+  const bool one = big || (per_step == 16 && p.tm + p.tn > 128) || (!a16 && p.tm == 128);
+  int64_t slabs = ((one ? 256 : 512) + mt * nt - 1) / (mt * nt);
   slabs = std::max(std::min(slabs, (steps * per_step + 31) / 32), (int64_t)1);
   p.mtiles = (int)mt; p.ntiles = (int)nt; p.chunks = (int)std::max(chunks, (int64_t)1);
   p.steps_per_slab = std::max(((int)((steps + slabs - 1) / slabs) + 1) & ~1, 2);
