@@ -8,12 +8,21 @@ mkdir -p "$OUT"
 cd "$OUT"
 # the build id the loader checks (csn_build_sources_sha16, include/csnet_hip.h): the unit sod100k_amd/_native.py generates
 python3 -c "import sys; sys.path.insert(0, '$HERE/../..'); from sod100k_amd import _native as N; N.write_build_id_object(N.hipcc_path(), N.sources_sha16(), '$OUT')"
-# sources and flags of the product build, linked aside so that a failed build leaves the library in the tree alone
-SRCS=$(python3 -c "import sys; sys.path.insert(0, '$HERE/../..'); from sod100k_amd import _native as N; print(*('$HERE/' + s for s in N.SOURCES))")
-FLAGS=$(python3 -c "import sys; sys.path.insert(0, '$HERE/../..'); from sod100k_amd import _native as N; print(*N.HIPCC_FLAGS)")
-hipcc $FLAGS -shared -Wl,--no-undefined -Rpass-analysis=kernel-resource-usage -save-temps -I"$HERE" \
-  -o "$OUT/libcsnet_hip.so" $SRCS "$OUT/csn_build_id.o" \
-  > "$OUT/build.log" 2>&1 || { cat "$OUT/build.log" | grep -E "error" -A3 | head -40; exit 1; }
+# sources and flags of the product build; linked aside, so that a failed build leaves the library in the tree alone
+py() { python3 -c "import sys; sys.path.insert(0, '$HERE/../..'); from sod100k_amd import _native as N; print(*$1)"; }
+FLAGS=$(py N.HIPCC_FLAGS)
+objs=""; jobs=""
+for s in $(py N.SOURCES); do
+  hipcc $FLAGS -Rpass-analysis=kernel-resource-usage -save-temps=obj -I"$HERE" -c "$HERE/$s" -o "$OUT/${s%.hip}.o" > "$OUT/${s%.hip}.log" 2>&1 &
+  jobs="$jobs $!"; objs="$objs $OUT/${s%.hip}.o"
+done
+failed=0
+for j in $jobs; do wait $j || failed=1; done
+cat "$OUT"/*.log > "$OUT/build.log.new"; mv "$OUT/build.log.new" "$OUT/build.log"
+if [ $failed = 0 ]; then
+  hipcc --offload-arch=gfx950 -shared -Wl,--no-undefined -o "$OUT/libcsnet_hip.so" $objs "$OUT/csn_build_id.o" >> "$OUT/build.log" 2>&1 || failed=1
+fi
+[ $failed = 0 ] || { grep -E "error|undefined" -A3 "$OUT/build.log" | head -40; exit 1; }
 cp "$OUT/libcsnet_hip.so" "$HERE/libcsnet_hip.so.new" && mv "$HERE/libcsnet_hip.so.new" "$HERE/libcsnet_hip.so"
 python3 - "$OUT/build.log" <<'PY'
 import re, sys
