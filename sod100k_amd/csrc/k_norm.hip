@@ -160,20 +160,22 @@ __device__ __forceinline__ void norm_param(float (&f)[E], const float* p, int n,
   }
 }
 
-// A float sum leaves a mean m off by some of its last places; the second pass, over x - m, finds out by how much.
+// The mean m of float channels, from a sum that rounds, is off by some of the last places of the largest; where the channels are close
+// together that shows.  The second pass, over x - m, finds out by how much.  (bfloat16 channels that are close together have an exact sum.)
 // The product that gives m must not be contracted with the subtraction: what is taken off would not be m.
 __device__ __forceinline__ float norm_first_mean(float sum, float inv_c) {
   unsigned m = csn_f_bits(sum * inv_c);
   csn_pin(m);
   return csn_bits_f(m);
 }
-// From the sums of (x - m)^2 and of x - m: the variance, and m becomes the mean.  (Equal channels: x - m is the same few last places of x for
-// all of them; sums, the quotient -- corrected once, a division at less cost -- and the difference are exact: mean x, variance 0.)
+// From the sums of (x - m)^2 and of x - m: the variance, and m becomes the mean where it is off by more than the second sum's own rounding,
+// counted as 2^-21 of the spread.  (Equal channels: x - m is the same few last places of x for all of them; sums, the quotient --
+// corrected once, a division at less cost -- and the difference are exact: mean x, variance 0.)
 __device__ __forceinline__ float norm_correct(float& m, float sq, float sum, float channels, float inv_c) {
-  const float q = sum * inv_c, off = fmaf(fmaf(-q, channels, sum), inv_c, q);
+  const float q = sum * inv_c, off = fmaf(fmaf(-q, channels, sum), inv_c, q), far = off * 2097152.f;
+  if (!(far * far > sq * inv_c)) return sq * inv_c;
   m += off;
-  const float var = fmaf(-off, sum, sq) * inv_c;
-  return var < 0.f ? 0.f : var;   // (a NaN stays one)
+  return fmaxf(fmaf(-off, sum, sq) * inv_c, 0.f);
 }
 
 template <int G> struct NormRowsBlock { static constexpr int T = G > CSN_BLOCK ? G : CSN_BLOCK; };
@@ -220,7 +222,9 @@ __global__ __launch_bounds__(NormRowsBlock<G>::T) void norm_rows_fwd_kernel(Norm
       for (int j = 0; j < E; ++j) s[0] += f[j];
     }
     norm_sum<G, 1>(s, sm, turn);
-    float mean = norm_first_mean(s[0], inv_c), d2[2] = {0.f, 0.f};
+    constexpr bool FIX = sizeof(AT) == 4;
+    float mean = FIX ? norm_first_mean(s[0], inv_c) : s[0] / (float)C, d2[FIX ? 2 : 1];   // (divided: equal channels have no variance at all)
+    d2[0] = d2[FIX] = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       float f[E];
@@ -230,11 +234,11 @@ __global__ __launch_bounds__(NormRowsBlock<G>::T) void norm_rows_fwd_kernel(Norm
       for (int j = 0; j < E; ++j) {
         const float d = j < n[v] ? f[j] - mean : 0.f;
         d2[0] = fmaf(d, d, d2[0]);
-        d2[1] += d;
+        if (FIX) d2[FIX] += d;
       }
     }
-    norm_sum<G, 2>(d2, sm, turn);
-    const float var = norm_correct(mean, d2[0], d2[1], (float)C, inv_c);
+    norm_sum<G, FIX ? 2 : 1>(d2, sm, turn);
+    const float var = FIX ? norm_correct(mean, d2[0], d2[FIX], (float)C, inv_c) : d2[0] * inv_c;
     const float rstd = 1.f / sqrtf(var + a.eps);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -385,7 +389,7 @@ __global__ __launch_bounds__(NormRowsBlock<G>::T) void norm_rows_bwd_kernel(Norm
 
 // Planar maps: PX lanes along the pixels (four consecutive pixels of a channel per lane: eight would double the statistics that
 // every lane carries), T / PX groups of lanes over the channels, NC channels per lane in registers.  Sums over a pixel's channels: butterfly over the groups of a wave, then the waves in
-// order through LDS (two buffers of [waves][2][PX * E] floats in turn).
+// order through LDS (two buffers of [waves][N][PX * E] floats in turn).
 #define NORM_PE 4
 template <int T, int PX, int E, int N>
 __device__ __forceinline__ void norm_planar_sum(float (&v)[N][E], float* sm, int& turn) {
@@ -401,8 +405,7 @@ __device__ __forceinline__ void norm_planar_sum(float (&v)[N][E], float* sm, int
       if (PX <= 2) v[i][j] += csn_lane_xor_f32<2>(v[i][j]);
     }
   if (W == 1) return;
-  static_assert(N <= 2, "a buffer holds two sums");
-  float* b = sm + turn * (W * 2 * TP);
+  float* b = sm + turn * (W * N * TP);
   turn ^= 1;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, px = lane % PX;
   if (lane < PX)
@@ -490,16 +493,13 @@ __global__ __launch_bounds__(T, 4) void norm_planar_fwd_kernel(NormArgs a) {
       CSN_SCHED_FENCE();   // one channel's floats at a time in registers
     }
     norm_planar_sum<T, PX, E, 1>(s, sm, turn);
-    // (As above; both sums of the second pass at once where the registers hold them.  float, whose channels take twice as many, would
-    // spill and corrects the mean in a pass of its own: at once / in turn, us, bf16 32x256x88x88 47.7 / 50.3, 16x512x44x44 16.1 / 17.0;
-    // float 16x2048x28x28 57.2 / 51.9, 16x1024x32x32 34.0 / 29.9, 32x256x88x88 107.6 / 105.4.)
-    constexpr bool ONCE = sizeof(AT) == 2;
+    // (As above; float channels leave no registers for both sums of the second pass at once, so the mean is corrected in a pass of its own:
+    // at once / in turn, us, 16x2048x28x28 57.2 / 51.9, 16x1024x32x32 34.0 / 29.9, 32x256x88x88 107.6 / 105.4.)
+    constexpr bool FIX = sizeof(AT) == 4;
     float mean[E], rstd[E];
 #pragma unroll
-    for (int j = 0; j < E; ++j) mean[j] = norm_first_mean(s[0][j], inv_c);
-    if constexpr (!ONCE) {
-#pragma unroll
-      for (int j = 0; j < E; ++j) s[0][j] = 0.f;
+    for (int j = 0; j < E; ++j) { mean[j] = FIX ? norm_first_mean(s[0][j], inv_c) : s[0][j] / (float)C; s[0][j] = 0.f; }
+    if constexpr (FIX) {
 #pragma unroll
       for (int k = 0; k < NC; ++k) {
         float f[E];
@@ -511,11 +511,8 @@ __global__ __launch_bounds__(T, 4) void norm_planar_fwd_kernel(NormArgs a) {
       }
       norm_planar_sum<T, PX, E, 1>(s, sm, turn);
 #pragma unroll
-      for (int j = 0; j < E; ++j) mean[j] = fmaf(s[0][j], inv_c, mean[j]);
+      for (int j = 0; j < E; ++j) { mean[j] = fmaf(s[0][j], inv_c, mean[j]); s[0][j] = 0.f; }
     }
-    float d2[ONCE ? 2 : 1][E];
-#pragma unroll
-    for (int j = 0; j < E; ++j) d2[0][j] = d2[ONCE][j] = 0.f;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       float f[E];
@@ -524,17 +521,13 @@ __global__ __launch_bounds__(T, 4) void norm_planar_fwd_kernel(NormArgs a) {
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         const float d = cg + CG * k < C ? f[j] - mean[j] : 0.f;
-        d2[0][j] = fmaf(d, d, d2[0][j]);
-        if (ONCE) d2[ONCE][j] += d;
+        s[0][j] = fmaf(d, d, s[0][j]);
       }
       CSN_SCHED_FENCE();
     }
-    norm_planar_sum<T, PX, E, ONCE ? 2 : 1>(d2, sm, turn);
+    norm_planar_sum<T, PX, E, 1>(s, sm, turn);
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const float var = ONCE ? norm_correct(mean[j], d2[0][j], d2[ONCE][j], (float)C, inv_c) : d2[0][j] * inv_c;
-      rstd[j] = 1.f / sqrtf(var + a.eps);
-    }
+    for (int j = 0; j < E; ++j) rstd[j] = 1.f / sqrtf(fmaf(s[0][j], inv_c, a.eps));
     const int64_t row0 = (int64_t)o * C;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
@@ -768,7 +761,7 @@ static int norm_rows_run(const NormArgs& a, const NormPlan& p, bool bwd, void* s
 }
 template <typename AT, int T, int PX, int NC, int CK>
 static int norm_planar_fwd(const NormArgs& a, void* stream) {
-  const size_t sm = (size_t)2 * (T / 64) * 2 * PX * NORM_PE * sizeof(float);
+  const size_t sm = (size_t)2 * (T / 64) * PX * NORM_PE * sizeof(float);
   CSN_LAUNCH((norm_planar_fwd_kernel<AT, T, PX, NC, CK>), dim3((unsigned)a.slabs), dim3(T), sm, stream, a);
   return (int)hipGetLastError();
 }
