@@ -134,6 +134,7 @@ class Engine:
         self.n_acts = len(acts)
         nbytes = int(lib.csn_plan_workspace_bytes(plan))
         self.workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+        self.params: Optional[torch.Tensor] = None  # keep_params(): the arena as the forward in the workspace saw it
         self._used, self._used_on = None, None      # of a training plan: event behind its last launch and the stream of that launch
 
     def __del__(self):
@@ -163,8 +164,9 @@ class Engine:
             self._used = torch.cuda.Event()
         elif self._used_on != stream.cuda_stream:
             stream.wait_event(self._used)
-            if self.workspace.is_cuda:              # (allocated on the stream of the plan's first call)
-                self.workspace.record_stream(stream)
+            for t in (self.workspace, self.params):  # (allocated on the stream of the plan's first call)
+                if t is not None and t.is_cuda:
+                    t.record_stream(stream)
         try:
             yield
         finally:                                    # (also where a call failed half way)
@@ -211,6 +213,21 @@ class Engine:
             N.check(self.lib, self.lib.csn_backward(self.plan, x.data_ptr(), dy.data_ptr(), self.workspace.data_ptr(),
                                                     arena.data_ptr(), grad.data_ptr(), grad.numel(), fw,
                                                     float(pen_scale), self._stream()), "csn_backward")
+
+    def keep_params(self, arena: torch.Tensor) -> None:
+        """Copy the arena for the backward of the ``forward_train`` in the workspace (always the same memory: a step's launches are
+        replayed as long as their pointers stay)."""
+        with self._in_turn():
+            if self.params is None:
+                self.params = torch.empty_like(arena)
+            self.params.copy_(arena)
+            if arena.is_cuda:
+                arena.record_stream(torch.cuda.current_stream(self.device))
+
+    def saved_params(self) -> torch.Tensor:
+        """What ``keep_params`` kept, for a forward that makes room."""
+        with self._in_turn():
+            return self.params.clone()
 
     def checkpoint_save(self, format: int) -> torch.Tensor:
         """8-bit checkpoint (``_native.Q8_INT8`` / ``Q8_E4M3``) of the last ``forward_train``: what ``backward`` reads of it."""

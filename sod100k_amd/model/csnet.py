@@ -671,6 +671,7 @@ class _CSNetTrainFn(torch.autograd.Function):
         elif s.checkpoint is not None:
             _displace(eng)                              # the workspace may hold another forward that still waits
             eng.checkpoint_restore(s.checkpoint, s.format)
+            eng.keep_params(s.params)
             model._train_generation += 1                # (a forward without checkpoints in between is gone, too)
         else:
             raise RuntimeError("CSNet backward a second time through one forward: its saved tensors are gone")
@@ -678,7 +679,7 @@ class _CSNetTrainFn(torch.autograd.Function):
         if dy is None:
             dy = torch.zeros((ctx.x.shape[0], 1) + tuple(ctx.x.shape[2:]), dtype=torch.float32, device=ctx.x.device)
         flat = torch.zeros(arena.n_param_floats, dtype=torch.float32, device=ctx.x.device)
-        eng.backward(ctx.x.contiguous(), dy.contiguous(), s.params, flat, s.flop_tab, float(dpen) if dpen is not None else 0.0)
+        eng.backward(ctx.x.contiguous(), dy.contiguous(), eng.params, flat, s.flop_tab, float(dpen) if dpen is not None else 0.0)
         dx = eng.train_probe(0, "grad0") if ctx.input_grad else None
         model._want_input_grad = False
         grads = [flat[arena.offsets[n]:arena.offsets[n] + p.numel()].view(p.shape) if p.requires_grad else None
@@ -693,7 +694,8 @@ class _SavedForward:
     def __init__(self, model, x, format):
         self.engine, self.format, self.flop_tab, self.checkpoint = model.engine_for(x, train=True), format, model._flop_tab, None
         # csn_backward reads the normalisations' weights: the forward's, whatever is written past the counters below (param.data)
-        self.arena, self.params, self.versions = model._arena, model._arena.flat.clone(), _versions(model)
+        self.arena, self.params, self.versions = model._arena, None, _versions(model)
+        self.engine.keep_params(model._arena.flat)
         # float32 steps read the image batch again in the backward (bfloat16 ones keep a copy of their own, which is saved)
         self.x_version = None if self.engine.train_bf16 or x.is_inference() else x._version
         self.engine.waiting = weakref.ref(self)
@@ -703,7 +705,9 @@ def _displace(eng):
     """Make room in a plan's workspace: the forward that lies there and waits for its backward, if there is one, is saved."""
     waiting = eng.waiting() if getattr(eng, "waiting", None) is not None else None
     if waiting is not None:
-        waiting.checkpoint = eng.checkpoint_save(waiting.format)   # (where this fails, out of memory say, it still lies there)
+        checkpoint = eng.checkpoint_save(waiting.format)           # (where this fails, out of memory say, it still lies there)
+        waiting.params = eng.saved_params()
+        waiting.checkpoint = checkpoint
     eng.waiting = None
 
 
