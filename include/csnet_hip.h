@@ -207,8 +207,8 @@ int csn_backward(csn_plan* plan, const float* x, const float* dy, void* workspac
  * activations, raw convolution outputs and pooled inputs as 8-bit checkpoints, one row per plane; the |GAP| tables, the bfloat16 copy of the
  * images and the packed tables as they are.  Taken after a csn_forward_train and before anything else writes the workspace, it lets
  * further forwards run on the plan before the first one's backward: restore it and call csn_backward with that forward's x (and
- * flop_w).  The gradients are those of the checkpoint's values.  Parameters must not change in between, as for any backward.
- * `checkpoint` is 256-byte aligned; launches on `stream`, no allocation. */
+ * flop_w) and parameters.  The gradients are those of the checkpoint's values.  A plan's calls share its workspace and its tables: on
+ * different streams the caller orders them.  `checkpoint` is 256-byte aligned; launches on `stream`, no allocation. */
 size_t csn_plan_checkpoint_bytes(const csn_plan* plan);   /* 0 before csn_plan_enable_training */
 int csn_plan_checkpoint_save(csn_plan* plan, const void* workspace, int32_t format, void* checkpoint, size_t checkpoint_bytes,
                              void* stream);

@@ -8,10 +8,12 @@
 // Bound by bytes: forward x and y, backward x, dy and dx, each once, at the 6.2 TB/s of a large copy.  A token's channels therefore stay in
 // registers over the passes that the formulas make (sum, sum of squares, output; the two sums of the backward, output), which are
 // lane exchanges and one trip through LDS.  Kernel times against that floor, us (cold caches):
-//   25088 x 512 float         forward 22.2 of 16.6   backward 28.2 of 24.8, sum of the slabs 4.0
-//   32x256x88x88 bf16         forward 49.3 of 40.9   backward 99   of 61.3, sum of the slabs 4.8
-//   16384 x 1024 bf16, int8 checkpoint    forward 21.5 of 13.6   backward 25.4 of 13.6, sum of the slabs 4.0
-//   16x512x44x44 float, e4m3 checkpoint   forward 35.2 of 23.1   backward 42.2 of 23.1, sum of the slabs 5.1
+//   25088 x 512 float         forward 22.7 of 16.6   backward 28.8 of 24.8, sum of the slabs 4.0
+//   16384 x 1024 bf16         forward 17.2 of 10.8   backward 23.7 of 16.2, sum of the slabs 4.0
+//   16384 x 1024 bf16, int8 checkpoint    forward 21.9 of 13.6   backward 25.6 of 13.6, sum of the slabs 4.0
+//   32x256x88x88 bf16         forward 48.7 of 40.9   backward 98.5 of 61.3, sum of the slabs 4.7
+//   32x256x88x88 float        forward 101.5 of 81.8  backward 158.5 of 123, sum of the slabs 4.8
+//   16x512x44x44 float, e4m3 checkpoint   forward 36.6 of 23.1   backward 42.2 of 23.1, sum of the slabs 4.0
 // The forward of maps waits for its loads between blocks (no room for the next tile beside 16 channels); the backward has the next tile
 // in flight, and what is left is the arithmetic and the exchanges between a tile's loads and its stores, two waves per SIMD.
 #include "csn_reduce.h"
