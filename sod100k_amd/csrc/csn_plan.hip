@@ -180,6 +180,7 @@ struct csn_plan {
   CsnPrepJob* jobs_dev = nullptr;
   bool params_ready = false;
   bool bn_tables_train = false;   // csn_forward_train overwrote the folded BN tables: refresh before eval
+  bool trained = false;           // a csn_forward_train has run: there may be checkpoints of it
   bool fuse_dw = true;
   bool fuse_cls = true;   // CSN_OPT_FUSE_CLS
   bool tiled3 = true;     // CSN_OPT_TILED3
@@ -2345,7 +2346,7 @@ int csn_forward_train(csn_plan* P, const float* x, float* y, void* workspace, fl
   if (!P || !x || !y || !workspace || !arena || !flop_w || !penalty) return CSN_E_INVALID;
   if (!P->params_ready) return CSN_E_STATE;
   (void)arena_floats;
-  P->bn_tables_train = true;   // host-side state: set here, a graph replay does not run the body
+  P->bn_tables_train = P->trained = true;   // host-side state: set here, a graph replay does not run the body
   const std::vector<uint64_t> key = {(uint64_t)(uintptr_t)x, (uint64_t)(uintptr_t)y, (uint64_t)(uintptr_t)workspace,
                                      (uint64_t)(uintptr_t)arena, (uint64_t)(uintptr_t)penalty,
                                      hash_floats(flop_w, (int)P->units.size() * CSN_MAX_BRANCH)};

@@ -135,8 +135,9 @@ int csn_plan_checkpoint_save(csn_plan* P, const void* workspace, int32_t format,
 int csn_plan_checkpoint_restore(csn_plan* P, void* workspace, int32_t format, const void* checkpoint, size_t checkpoint_bytes, void* stream) {
   REFUSE_UNLINKED();
   if (!P || !workspace || !checkpoint || ((uintptr_t)checkpoint & 255u) || !format_ok(format)) REFUSE("plan checkpoint: null or misaligned (256 bytes) buffer, unknown format");
-  if (!P->train || !P->bn_tables_train) { g_hip_err = "plan checkpoint: a training plan that has run a forward is needed"; return CSN_E_STATE; }
+  if (!P->train || !P->trained) { g_hip_err = "plan checkpoint: a training plan that has run a forward is needed"; return CSN_E_STATE; }
   if (checkpoint_bytes < (size_t)plan_saved_bytes(P)) REFUSE("plan checkpoint: buffer smaller than csn_plan_checkpoint_bytes");
+  P->bn_tables_train = true;   // (the packed tables are among what comes back, whatever refreshed them since)
   return plan_saved_move(P, static_cast<char*>(workspace), static_cast<char*>(const_cast<void*>(checkpoint)), format, false, stream);
 }
 

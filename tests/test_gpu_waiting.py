@@ -37,3 +37,7 @@ def test_gpu_failed_save(lib, x2_manifest):
 @pytest.mark.parametrize("act_dtype", ["fp32", "bf16"])
 def test_gpu_penalty_and_input_gradients(lib, x2_manifest, act_dtype):
     W.check_penalty_and_input_gradients(lib, DEV, x2_manifest, act_dtype, B=3, size=48)
+
+
+def test_gpu_failed_forward(lib, x2_manifest):
+    W.check_failed_forward(lib, DEV, x2_manifest)

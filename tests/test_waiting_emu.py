@@ -89,3 +89,7 @@ def test_emu_failed_save(lib, x2_manifest):
 
 def test_emu_penalty_and_input_gradients(lib, x2_manifest):
     W.check_penalty_and_input_gradients(lib, CPU, x2_manifest, "fp32")
+
+
+def test_emu_failed_forward(lib, x2_manifest):
+    W.check_failed_forward(lib, CPU, x2_manifest)

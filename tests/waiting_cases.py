@@ -168,3 +168,27 @@ def check_penalty_and_input_gradients(lib, device, manifest, act_dtype, B=2, siz
     assert torch.equal(leaves[0].grad, dx0) and torch.equal(leaves[1].grad, dx1)
     assert torch.equal(grads(m), g1 + g0)
     assert bool(dx0.abs().sum() > 0) and not torch.equal(g0, g1)
+
+
+def check_failed_forward(lib, device, manifest):
+    """A forward that fails after it has made room (its parameters are packed already): the one that waits still has its checkpoint."""
+    xs = [batch(s, device) for s in (31, 32)]
+    dy = K.gradient((1, 1, 16, 16), torch.float32, 1, device)
+    m = net(lib, device, manifest)
+    a, b = m(xs[0]), m(xs[1])
+    a.backward(dy)
+    want = grads(m)
+    del b
+    a = m(xs[0])
+    eng = m.engine_for(xs[1], train=True)
+    forward = eng.forward_train
+
+    def fails(*args, **kwargs):
+        raise torch.OutOfMemoryError("no room")
+    eng.forward_train = fails
+    with pytest.raises(torch.OutOfMemoryError):
+        m(xs[1])
+    eng.forward_train = forward
+    a.backward(dy)
+    assert torch.equal(grads(m), want)
+    m(xs[1]).backward(dy)                    # and the plan goes on
